@@ -15,6 +15,7 @@ DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 BYTES = {"f32": 4, "bf16": 2, "f16": 2}
 CLIP, ENTROPY_COEF, KL_COEF = 0.2, 0.01, 0.05          # clip of the ratio, weight of the entropy, weight of the KL term
 VALUE_CLIP, HUBER_DELTA = 0.2, 10.0
+GRAD_SCALE = {"f32": 1.0, "bf16": 1.0, "f16": 1024.0}  # loss scaling: the mean over many rows leaves gradients below the range of f16
 # the reference-architecture network on the 5 x 4 grid: conv 20 -> 32, 192 -> 64, 64 -> 64, head of 6
 NETWORK = [(32, 20, 3, 3), (32,), (64, 192), (64,), (64, 64), (64,), (6, 64), (6,)]
 
@@ -212,6 +213,7 @@ def prepare(case, seed):
     state["case"] = case
     if case.get("how") == "autograd":
         state["logits" if case["op"] == "policy_loss" else "values"].requires_grad_()
+        state["scale"] = torch.tensor(GRAD_SCALE[case["dtype"]], device="cuda")
     if case.get("how") == "train":
         for leaf in ("x", "weight", "bias"):
             state[leaf].requires_grad_()
@@ -258,6 +260,7 @@ def _plain_policy(s):
     out = [loss, torch.stack(means)]
     if case["how"] == "forward":
         return out
+    w = w * GRAD_SCALE[case["dtype"]]
     grad = (w * slope).unsqueeze(1) * (torch.zeros_like(p).scatter_(1, at, 1.0) - p)
     grad += (w * ENTROPY_COEF).unsqueeze(1) * p * (logp + entropy.unsqueeze(1))
     return out + [torch.where(counts.unsqueeze(1) & possible, grad, 0.0).to(s["logits"].dtype)]
@@ -279,7 +282,7 @@ def _plain_value(s):
     out = [(w * torch.maximum(h0, h1)).sum()]
     if s["case"]["how"] == "forward":
         return out
-    return out + [torch.where(((v - v0).abs() <= VALUE_CLIP) | (h0 >= h1), -w * slope, 0.0).to(s["values"].dtype)]
+    return out + [torch.where(((v - v0).abs() <= VALUE_CLIP) | (h0 >= h1), -w * slope * GRAD_SCALE[s["case"]["dtype"]], 0.0).to(s["values"].dtype)]
 
 
 def _plain_clip(s):
@@ -318,9 +321,9 @@ def _own_policy(s):
     kw = dict(clip_param=CLIP, entropy_coef=ENTROPY_COEF, kl_coef=KL_COEF, ref_log_probs=s["ref"], active_masks=s["weights"],
               available_actions=s["avail"])
     if how == "grad":
-        return list(dc.policy_loss_grad(*args, **kw))
+        return list(dc.policy_loss_grad(*args, grad_scale=GRAD_SCALE[s["case"]["dtype"]], **kw))
     loss, stats = dc.policy_loss(*args, **kw)
-    return [loss, stats] if how == "forward" else [loss.detach(), stats, torch.autograd.grad(loss, s["logits"])[0]]
+    return [loss, stats] if how == "forward" else [loss.detach(), stats, torch.autograd.grad(loss, s["logits"], s["scale"])[0]]
 
 
 def _own_value(s):
@@ -330,9 +333,9 @@ def _own_value(s):
     kw = dict(clip_param=VALUE_CLIP, huber_delta=HUBER_DELTA if s["case"]["huber"] else None, active_masks=s["weights"],
               value_normalizer=s["norm"])
     if how == "grad":
-        return list(dc.value_loss_grad(*args, **kw))
+        return list(dc.value_loss_grad(*args, grad_scale=GRAD_SCALE[s["case"]["dtype"]], **kw))
     loss = dc.value_loss(*args, **kw)
-    return [loss] if how == "forward" else [loss.detach(), torch.autograd.grad(loss, s["values"])[0]]
+    return [loss] if how == "forward" else [loss.detach(), torch.autograd.grad(loss, s["values"], s["scale"])[0]]
 
 
 def _own_clip(s):
@@ -412,7 +415,7 @@ def _exact_policy(case, s):
     means = torch.stack([(share * t).sum() for t in (pol, entropy, kl, outside, ratio)])
     loss = means[0] - ENTROPY_COEF * means[1] + KL_COEF * means[2]
     out = [loss.detach(), means.detach()]
-    return out if case["how"] == "forward" else out + [torch.autograd.grad(loss, z)[0]]
+    return out if case["how"] == "forward" else out + [torch.autograd.grad(loss * GRAD_SCALE[case["dtype"]], z)[0]]
 
 
 def _exact_value(case, s):
@@ -429,7 +432,7 @@ def _exact_value(case, s):
 
     worst = torch.max(h(target - v), h(target - v0 - (v - v0).clamp(-VALUE_CLIP, VALUE_CLIP)))
     loss = (w * worst).sum() / w.sum().clamp(min=1e-300)
-    return [loss.detach()] if case["how"] == "forward" else [loss.detach(), torch.autograd.grad(loss, v)[0]]
+    return [loss.detach()] if case["how"] == "forward" else [loss.detach(), torch.autograd.grad(loss * GRAD_SCALE[case["dtype"]], v)[0]]
 
 
 def _exact_clip(case, s):
