@@ -407,7 +407,7 @@ std::string sm1f_batch(int sm) {
 constexpr const char *kJitPreloadOption = "-amdgpu-kernarg-preload-count=14";
 
 std::string jit_prologue() {
-    std::string t = std::string("// hiprtc options: -O3 -std=c++17 -mllvm ") + kJitPreloadOption + "\n#define OC_JIT 1\n";
+    std::string t = std::string("// hiprtc options: -O3 -std=c++17 -packed-fp32-ops -mllvm ") + kJitPreloadOption + "\n#define OC_JIT 1\n";
     if (const char *nu = OC_DIAG_ENV("OC_NOUNROLL")) t += std::string("#define OC_NOUNROLL ") + ((nu[0] && nu[0] != '0') ? "1\n" : "0\n");
     // (batched flush: on by default for grids of at most 32 tiles, see oc_step_body.h; the environment overrides)
     if (const char *ff = OC_DIAG_ENV("OC_FAST_FLUSH")) t += std::string("#define OC_FAST_FLUSH ") + ((ff[0] && ff[0] != '0') ? "1\n" : "0\n");
@@ -758,8 +758,8 @@ int jit_compile_text(const std::string &text, const char *arch, std::vector<char
         return OC_ERR_HIP;
     }
     const std::string archopt = std::string("--offload-arch=") + arch;
-    const char *copts[] = {archopt.c_str(), "-O3", "-std=c++17", "-mllvm", kJitPreloadOption};
-    const hiprtcResult r = hiprtcCompileProgram(prog, 5, copts);
+    const char *copts[] = {archopt.c_str(), "-O3", "-std=c++17", "-mllvm", kJitPreloadOption, "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};
+    const hiprtcResult r = hiprtcCompileProgram(prog, sizeof(copts) / sizeof(copts[0]), copts);
     size_t n = 0;
     if (hiprtcGetProgramLogSize(prog, &n) == HIPRTC_SUCCESS && n > 1) { log.resize(n); hiprtcGetProgramLog(prog, &log[0]); }
     int rc = OC_OK;
