@@ -1,0 +1,1022 @@
+// update_ops.hip -- what a policy-gradient update computes behind the rollout, gfx950: the clipped policy loss over logits and the clipped
+// value loss, each with its gradient, and the global norm of many gradient tensors with clipping.  All of it streams: each operator is
+// bound by the bytes of its inputs and outputs, and is built to read every input once (the gradient norm: once per pass).
+//
+// Sums over rows are kept in f64 and added in a fixed order (per-block partial sums, no atomics): the results do not depend on which
+// block ran when.  Everything inside a row is f32, whatever the logits' type; a gradient is rounded once, to the logits' type.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "overcooked_ops.h"
+#include "oc_internal.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// a 16-byte access at an element's own alignment: rows of an odd number of 2-byte elements start anywhere, and global memory
+// instructions take any address
+typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
+
+template <int ALIGN> struct Unaligned { typedef u32x4_a4 type; };
+template <> struct Unaligned<2> { typedef u32x4_a2 type; };
+
+template <typename T> struct Chunk {                       // 16 bytes of elements
+    static constexpr int V = 16 / sizeof(T);
+    union { u32x4 raw; T e[V]; };
+    __device__ Chunk() {}
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -1e30f;                          // floor of log-probabilities in products with a probability of 0
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr int kMaxBlocks = 2048;                           // of a launch that leaves one set of partial sums per block
+constexpr int kWeightBlocks = 256;                         // of the launch that adds up the weights
+constexpr int kSums = 6;
+
+struct PolicyLossArgs {
+    const void *logits;
+    const void *actions;
+    const float *old_logp, *adv, *ref_logp, *weights;      // ref_logp, weights: or NULL
+    const void *avail;                                     // or NULL
+    void *grad;
+    const float *grad_out;                                 // upstream gradient (device) or NULL = 1
+    float *loss, *stats;                                   // [1], [5] or NULL
+    double *weight;                                        // W: written by a forward pass, read by the backward pass
+    double *weight_partials;                               // [kWeightBlocks]
+    double *sums;                                          // [blocks][kSums]
+    long long rows, row_stride, avail_stride;
+    int n_actions, action_type, avail_u8;
+    int weight_from;                                       // of the weight: see enum
+    int n_weight_partials, finalize_here, want_sums;
+    float clip_lo, clip_hi, entropy_coef, kl_coef, grad_scale;
+};
+// where a block takes the total weight from: nowhere (no gradient: the sums carry it), every block adds it up itself (few rows), the
+// partial sums of the launch before, what the forward pass has left
+enum { WEIGHT_NONE = 0, WEIGHT_SELF = 1, WEIGHT_PARTIALS = 2, WEIGHT_GIVEN = 3 };
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+// Sum over the block, valid in every thread; `part`: LDS, one double per wavefront.
+__device__ __forceinline__ double block_sum(double x, double *part) {
+    x = wave_sum(x);
+    const int waves = blockDim.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = part[0];
+    for (int w = 1; w < waves; ++w) x += part[w];
+    return x;
+}
+
+// The taken action of a row, -1 when it is none of 0 .. n - 1 (also a float that is NaN or lies outside).
+__device__ __forceinline__ int action_of(const PolicyLossArgs &a, long long row) {
+    long long v;
+    if (a.action_type == OC_ACT_F32) {
+        const float f = static_cast<const float *>(a.actions)[row];
+        v = f > -1.0f && f < static_cast<float>(a.n_actions) ? static_cast<long long>(f) : -1;
+    } else if (a.action_type == OC_ACT_I64) {
+        v = static_cast<const long long *>(a.actions)[row];
+    } else {
+        v = static_cast<const int *>(a.actions)[row];
+    }
+    return v >= 0 && v < a.n_actions ? static_cast<int>(v) : -1;
+}
+
+__device__ __forceinline__ double row_weight(const PolicyLossArgs &a, long long row) {
+    if (action_of(a, row) < 0) return 0.0;
+    return a.weights ? static_cast<double>(a.weights[row]) : 1.0;
+}
+
+__global__ __launch_bounds__(256) void oc_policy_weight_kernel(const PolicyLossArgs a) {
+    __shared__ double part[4];
+    double w = 0.0;
+    const long long stride = static_cast<long long>(gridDim.x) * 256;
+    for (long long r = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; r < a.rows; r += stride) w += row_weight(a, r);
+    w = block_sum(w, part);
+    if (threadIdx.x == 0) a.weight_partials[blockIdx.x] = w;
+}
+
+// 1 / total weight, 0 when there is none.
+__device__ __forceinline__ float inverse_weight(const PolicyLossArgs &a, double *part) {
+    double w = 0.0;
+    if (a.weight_from == WEIGHT_SELF) {
+        for (long long r = threadIdx.x; r < a.rows; r += blockDim.x) w += row_weight(a, r);
+        w = block_sum(w, part);
+    } else if (a.weight_from == WEIGHT_PARTIALS) {
+        for (int i = threadIdx.x; i < a.n_weight_partials; i += blockDim.x) w += a.weight_partials[i];
+        w = block_sum(w, part);
+    } else if (a.weight_from == WEIGHT_GIVEN) {
+        w = *a.weight;
+    }
+    return w != 0.0 ? static_cast<float>(1.0 / w) : 0.0f;
+}
+
+// What the rows of a thread (or of a group's first lane) add to the sums.
+struct RowSums {
+    double policy = 0, entropy = 0, kl = 0, clipped = 0, ratio = 0, weight = 0;
+};
+
+__device__ __forceinline__ void write_result(const PolicyLossArgs &a, const double (&s)[kSums]) {
+    const double inv = s[5] != 0.0 ? 1.0 / s[5] : 0.0;
+    double loss = s[0];                                    // a term without weight stays out, also where it is not finite
+    if (a.entropy_coef != 0.0f) loss -= static_cast<double>(a.entropy_coef) * s[1];
+    if (a.kl_coef != 0.0f) loss += static_cast<double>(a.kl_coef) * s[2];
+    *a.loss = static_cast<float>(loss * inv);
+    if (a.stats)
+#pragma unroll
+        for (int i = 0; i < 5; ++i) a.stats[i] = static_cast<float>(s[i] * inv);
+    if (a.weight) *a.weight = s[5];
+}
+
+__device__ __forceinline__ void finish_sums(const PolicyLossArgs &a, const RowSums &r, double *part) {
+    if (!a.want_sums) return;
+    double s[kSums] = {r.policy, r.entropy, r.kl, r.clipped, r.ratio, r.weight};
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) s[i] = block_sum(s[i], part);
+    if (threadIdx.x != 0) return;
+    if (a.finalize_here) {
+        write_result(a, s);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) a.sums[static_cast<long long>(blockIdx.x) * kSums + i] = s[i];
+    }
+}
+
+__global__ __launch_bounds__(256) void oc_policy_finalize_kernel(const PolicyLossArgs a, int blocks) {
+    __shared__ double part[4];
+    double s[kSums] = {0, 0, 0, 0, 0, 0};
+    for (int b = threadIdx.x; b < blocks; b += 256)
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) s[i] += a.sums[static_cast<long long>(b) * kSums + i];
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) s[i] = block_sum(s[i], part);
+    if (threadIdx.x == 0) write_result(a, s);
+}
+
+// One row behind its softmax: `za` the taken action's logit (-inf: not possible), m the largest logit, s = sum exp(z - m),
+// t = sum exp(z - m) (z - m).  Adds to the sums; the gradient of logit j is then p_j (ce (z_j - m) + k) + [j == taken] c1 with
+// p_j = exp(z_j - m) / s:
+//   d loss / d lp = c1 = (w / W) (-A ratio [not clipped] + ck (1 - exp(ref - lp)));  d H / d z_j = -p_j (log p_j + H).
+struct RowGrad { float c1, ce, k, inv_s; };
+
+__device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, long long row, float weight, float inv_w, float za, float m, float s, float t,
+                                             bool leader, RowSums &sums) {
+    RowGrad g = {0.0f, 0.0f, 0.0f, 0.0f};
+    // nothing is possible, or the taken action is not: the row adds nothing (logits that are all NaN leave m at -inf and s NaN)
+    if ((m == neg_inf() && s == 0.0f) || za == neg_inf()) return g;
+    const float log_s = logf(s);
+    const float lp = (za - m) - log_s;
+    const float entropy = log_s - t / s;
+    const float adv = a.adv[row];
+    const float ratio = expf(lp - a.old_logp[row]);
+    const float kept = fminf(fmaxf(ratio, a.clip_lo), a.clip_hi);
+    const float s1 = ratio * adv, s2 = kept * adv;
+    const float policy = -(s1 != s1 || s2 != s2 ? s1 + s2 : fminf(s1, s2));
+    const bool cut = (adv > 0.0f && ratio > a.clip_hi) || (adv < 0.0f && ratio < a.clip_lo);
+    float slope = cut ? 0.0f : -s1;
+    float kl = 0.0f;
+    if (a.ref_logp) {
+        const float d = a.ref_logp[row] - lp, e = expm1f(d);
+        kl = e - d;
+        if (a.kl_coef != 0.0f) slope = slope - a.kl_coef * e;
+    }
+    if (leader) {
+        const double w = weight;
+        sums.policy += w * policy;
+        sums.entropy += w * entropy;
+        sums.kl += w * kl;
+        sums.clipped += ratio < a.clip_lo || ratio > a.clip_hi ? w : 0.0;
+        sums.ratio += w * ratio;
+    }
+    const float scale = weight * inv_w;
+    g.c1 = scale * slope;
+    g.ce = scale * a.entropy_coef;
+    g.k = g.ce * (entropy - log_s) - g.c1;
+    g.inv_s = 1.0f / s;
+    return g;
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------
+// Up to 16 actions: a thread has a whole row.  The block's 256 rows are one contiguous piece of memory; it is copied through LDS in
+// 16-byte pieces, because lanes that each load their own 24 bytes touch every line of the piece once per load.  AM: 4, 8 or 16 values
+// are held in registers.
+// -------------------------------------------------------------------------------------------------------------------------------
+constexpr int kRowTile = 256;
+
+template <int ALIGN>
+__device__ __forceinline__ void copy_in(void *lds, const void *src, int bytes) {
+    typedef typename Unaligned<ALIGN>::type U;
+    const int whole = bytes & ~15;
+    for (int b = threadIdx.x * 16; b < whole; b += 256 * 16)
+        *reinterpret_cast<u32x4 *>(static_cast<char *>(lds) + b) = *reinterpret_cast<const U *>(static_cast<const char *>(src) + b);
+    if (static_cast<int>(threadIdx.x) < bytes - whole) static_cast<char *>(lds)[whole + threadIdx.x] = static_cast<const char *>(src)[whole + threadIdx.x];
+}
+
+template <int ALIGN>
+__device__ __forceinline__ void copy_out(void *dst, const void *lds, int bytes) {
+    typedef typename Unaligned<ALIGN>::type U;
+    const int whole = bytes & ~15;
+    for (int b = threadIdx.x * 16; b < whole; b += 256 * 16)
+        *reinterpret_cast<U *>(static_cast<char *>(dst) + b) = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(lds) + b);
+    if (static_cast<int>(threadIdx.x) < bytes - whole) static_cast<char *>(dst)[whole + threadIdx.x] = static_cast<const char *>(lds)[whole + threadIdx.x];
+}
+
+template <typename T, int AM, bool GRAD>
+__global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLossArgs a) {
+    __shared__ __attribute__((aligned(16))) T rows_lds[kRowTile * AM];
+    __shared__ __attribute__((aligned(16))) char avail_lds[kRowTile * AM * 4];
+    __shared__ double part[4];
+    const int A = a.n_actions;
+    const float inv_w = GRAD ? inverse_weight(a, part) : 0.0f;
+    const float go = GRAD ? a.grad_scale * (a.grad_out ? *a.grad_out : 1.0f) : 0.0f;
+    const bool stage_avail = a.avail && a.avail_stride == A;
+    RowSums sums;
+    const long long tiles = (a.rows + kRowTile - 1) / kRowTile;
+    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const long long row0 = tile * kRowTile;
+        const int n = static_cast<int>(a.rows - row0 < kRowTile ? a.rows - row0 : kRowTile);
+        const int me = threadIdx.x;
+        const long long row = row0 + me;
+        const bool live = me < n;
+        if (a.row_stride == A)
+            copy_in<sizeof(T) == 4 ? 4 : 2>(rows_lds, static_cast<const T *>(a.logits) + row0 * A, n * A * static_cast<int>(sizeof(T)));
+        else if (live)
+            for (int j = 0; j < A; ++j) rows_lds[me * A + j] = static_cast<const T *>(a.logits)[row * a.row_stride + j];
+        if (stage_avail) {
+            const int size = a.avail_u8 ? 1 : 4;
+            const char *src = static_cast<const char *>(a.avail) + row0 * A * size;
+            if (a.avail_u8) {
+                for (int b = me; b < n * A; b += 256) avail_lds[b] = src[b];
+            } else {
+                copy_in<4>(avail_lds, src, n * A * 4);
+            }
+        }
+        const int action = live ? action_of(a, row) : -1;
+        const float weight = action < 0 ? 0.0f : a.weights ? a.weights[row] : 1.0f;
+        __syncthreads();
+        float z[AM];
+        float m = neg_inf(), za = neg_inf();
+#pragma unroll
+        for (int j = 0; j < AM; ++j) {
+            z[j] = neg_inf();
+            if (j < A && live) {
+                bool may = true;
+                if (stage_avail)
+                    may = a.avail_u8 ? avail_lds[me * A + j] != 0 : reinterpret_cast<const float *>(avail_lds)[me * A + j] != 0.0f;
+                else if (a.avail)
+                    may = a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[row * a.avail_stride + j] != 0
+                                     : static_cast<const float *>(a.avail)[row * a.avail_stride + j] != 0.0f;
+                if (may) z[j] = static_cast<float>(rows_lds[me * A + j]);
+                if (j == action) za = z[j];
+            }
+            m = fmaxf(m, z[j]);
+        }
+        RowGrad g = {0.0f, 0.0f, 0.0f, 0.0f};
+        float s = 0.0f, t = 0.0f;
+        if (weight != 0.0f) {
+            sums.weight += weight;
+            const float base = m == neg_inf() ? 0.0f : m;
+#pragma unroll
+            for (int j = 0; j < AM; ++j) {
+                const float u = z[j] - base, e = exp2_fast(u * kLog2e);
+                s += e;
+                t = fmaf(e, fmaxf(u, kLowest), t);
+            }
+            g = row_terms(a, row, weight, inv_w, za, m, s, t, true, sums);
+        }
+        if (GRAD) {
+#pragma unroll
+            for (int j = 0; j < AM; ++j) {
+                if (j < A && live) {
+                    const float u = z[j] - m;
+                    float d = exp2_fast(u * kLog2e) * g.inv_s * fmaf(g.ce, fmaxf(u, kLowest), g.k) + (j == action ? g.c1 : 0.0f);
+                    if (g.inv_s == 0.0f || z[j] == neg_inf()) d = 0.0f;
+                    rows_lds[me * A + j] = static_cast<T>(d * go);
+                }
+            }
+            __syncthreads();
+            copy_out<sizeof(T) == 4 ? 4 : 2>(static_cast<T *>(a.grad) + row0 * A, rows_lds, n * A * static_cast<int>(sizeof(T)));
+        }
+        __syncthreads();
+    }
+    finish_sums(a, sums, part);
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------
+// More actions: L lanes have a row together, each C pieces of 16 bytes of it in registers (C = 0: more than fits, the row is read again
+// for the gradient).  One pass: a wavefront's maximum, its sums relative to that, and, where several wavefronts share the row, one
+// exchange of (maximum, sums) through LDS.
+// -------------------------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const PolicyLossArgs &a, const T *row_ptr, long long row, int c) {
+    constexpr int V = Chunk<T>::V;
+    typedef typename Unaligned<sizeof(T)>::type U;
+    Chunk<T> x;
+    const int j0 = c * V;
+    if (j0 + V <= a.n_actions) {
+        x.raw = *reinterpret_cast<const U *>(row_ptr + j0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x.e[i] = j0 + i < a.n_actions ? row_ptr[j0 + i] : static_cast<T>(neg_inf());
+    }
+    if (a.avail && j0 + V <= a.n_actions) {
+        if (a.avail_u8) {
+            const uint8_t *may = static_cast<const uint8_t *>(a.avail) + row * a.avail_stride + j0;
+            uint8_t bytes[V];
+            __builtin_memcpy(bytes, may, V);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (bytes[i] == 0) x.e[i] = static_cast<T>(neg_inf());
+        } else {
+            const float *may = static_cast<const float *>(a.avail) + row * a.avail_stride + j0;
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                const u32x4 four = reinterpret_cast<const u32x4_a4 *>(may)[q];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((four[i] << 1) == 0) x.e[q * 4 + i] = static_cast<T>(neg_inf());        // +0 or -0
+            }
+        }
+    } else if (a.avail) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (j0 + i < a.n_actions) {
+                const long long at = row * a.avail_stride + j0 + i;
+                const bool may = a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[at] != 0 : static_cast<const float *>(a.avail)[at] != 0.0f;
+                if (!may) x.e[i] = static_cast<T>(neg_inf());
+            }
+        }
+    }
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_grad(const PolicyLossArgs &a, long long row, int c, const Chunk<T> &x) {
+    constexpr int V = Chunk<T>::V;
+    typedef typename Unaligned<sizeof(T)>::type U;
+    T *dst = static_cast<T *>(a.grad) + row * a.n_actions + c * V;
+    if (c * V + V <= a.n_actions) {
+        *reinterpret_cast<U *>(dst) = x.raw;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (c * V + i < a.n_actions) dst[i] = x.e[i];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, float m, const RowGrad &g, float go) {
+    Chunk<T> y;
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::V; ++i) {
+        const float z = static_cast<float>(x.e[i]);
+        const float u = z - m;
+        float d = exp2_fast(u * kLog2e) * g.inv_s * fmaf(g.ce, fmaxf(u, kLowest), g.k) + (c * Chunk<T>::V + i == action ? g.c1 : 0.0f);
+        if (z == neg_inf()) d = 0.0f;
+        y.e[i] = static_cast<T>(d * go);
+    }
+    return y;
+}
+
+template <int W>
+__device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+    for (int off = W / 2; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
+    return x;
+}
+
+template <int W>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+    for (int off = W / 2; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_sums(const Chunk<T> &x, float base, float &s, float &t) {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::V; ++i) {
+        const float u = static_cast<float>(x.e[i]) - base, e = exp2_fast(u * kLog2e);
+        s += e;
+        t = fmaf(e, fmaxf(u, kLowest), t);
+    }
+}
+
+template <typename T, int L, int C, bool GRAD>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void oc_policy_loss_group_kernel(const PolicyLossArgs a) {
+    constexpr int B = L < 256 ? 256 : L;                   // threads of a block
+    constexpr int R = B / L;                               // rows of a block
+    constexpr int LW = L < 64 ? L : 64;                    // lanes of a wavefront that share a row
+    constexpr int NW = L / LW;                             // wavefronts that share a row
+    constexpr int V = Chunk<T>::V;
+    __shared__ float merge[2][NW][4];
+    __shared__ double part[B / 64];
+    const float inv_w = GRAD ? inverse_weight(a, part) : 0.0f;
+    const float go = GRAD ? a.grad_scale * (a.grad_out ? *a.grad_out : 1.0f) : 0.0f;
+    const int lane = threadIdx.x % L;
+    const int n_chunks = (a.n_actions + V - 1) / V;
+    RowSums sums;
+    int parity = 0;
+    for (long long row = static_cast<long long>(blockIdx.x) * R + threadIdx.x / L; row < a.rows; row += static_cast<long long>(gridDim.x) * R) {
+        const int action = action_of(a, row);
+        const float weight = action < 0 ? 0.0f : a.weights ? a.weights[row] : 1.0f;
+        if (weight == 0.0f) {
+            if (GRAD) {
+                Chunk<T> zero;
+                zero.raw = u32x4{0, 0, 0, 0};
+                for (int c = lane; c < n_chunks; c += L) store_grad<T>(a, row, c, zero);
+            }
+            continue;
+        }
+        const T *row_ptr = static_cast<const T *>(a.logits) + row * a.row_stride;
+        Chunk<T> x[C ? C : 1];
+        float m = neg_inf(), s = 0.0f, t = 0.0f;
+        if (C) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (lane + i * L < n_chunks) x[i] = load_chunk<T>(a, row_ptr, row, lane + i * L);
+        }
+        float za = static_cast<float>(row_ptr[action]);
+        if (a.avail) {
+            const long long at = row * a.avail_stride + action;
+            if (a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[at] == 0 : static_cast<const float *>(a.avail)[at] == 0.0f) za = neg_inf();
+        }
+        if (C) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (lane + i * L < n_chunks)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) m = fmaxf(m, static_cast<float>(x[i].e[k]));
+            m = lanes_max<LW>(m);
+            const float base = m == neg_inf() ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (lane + i * L < n_chunks) chunk_sums<T>(x[i], base, s, t);
+        } else {
+            // running maximum and sums of a lane, rescaled where a piece raises the maximum
+            for (int c = lane; c < n_chunks; c += L) {
+                const Chunk<T> y = load_chunk<T>(a, row_ptr, row, c);
+                float mc = m;
+#pragma unroll
+                for (int k = 0; k < V; ++k) mc = fmaxf(mc, static_cast<float>(y.e[k]));
+                if (mc > m) {
+                    if (m != neg_inf()) {
+                        const float f = exp2_fast((m - mc) * kLog2e);
+                        t = f * fmaf(s, m - mc, t);
+                        s *= f;
+                    }
+                    m = mc;
+                }
+                chunk_sums<T>(y, m == neg_inf() ? 0.0f : m, s, t);
+            }
+            const float mw = lanes_max<LW>(m);
+            if (mw > m && m != neg_inf()) {
+                const float f = exp2_fast((m - mw) * kLog2e);
+                t = f * fmaf(s, m - mw, t);
+                s *= f;
+            }
+            m = mw;
+        }
+        s = lanes_sum<LW>(s);
+        t = lanes_sum<LW>(t);
+        if (NW > 1) {
+            const int wave = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) { merge[parity][wave][0] = m; merge[parity][wave][1] = s; merge[parity][wave][2] = t; }
+            __syncthreads();
+            float mm = neg_inf();
+#pragma unroll
+            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, merge[parity][w][0]);
+            s = 0.0f;
+            t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float mw = merge[parity][w][0], sw = merge[parity][w][1], tw = merge[parity][w][2];
+                // a wavefront without a possible action has sums of 0 (or NaN, which has to reach the result)
+                const float f = mw == neg_inf() ? 1.0f : exp2_fast((mw - mm) * kLog2e);
+                s = fmaf(f, sw, s);
+                t = fmaf(f, mw == neg_inf() ? tw : fmaf(sw, fmaxf(mw - mm, kLowest), tw), t);
+            }
+            m = mm;
+            parity ^= 1;                                   // the next row's exchange does not overwrite one that is still read
+        }
+        if (lane == 0) sums.weight += weight;
+        const RowGrad g = row_terms(a, row, weight, inv_w, za, m, s, t, lane == 0, sums);
+        if (GRAD) {
+            const bool none = g.inv_s == 0.0f;
+            if (C) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    const int c = lane + i * L;
+                    if (c < n_chunks) {
+                        Chunk<T> y = grad_chunk<T>(x[i], c, action, m, g, go);
+                        if (none) y.raw = u32x4{0, 0, 0, 0};
+                        store_grad<T>(a, row, c, y);
+                    }
+                }
+            } else {
+                for (int c = lane; c < n_chunks; c += L) {
+                    Chunk<T> y = grad_chunk<T>(load_chunk<T>(a, row_ptr, row, c), c, action, m, g, go);
+                    if (none) y.raw = u32x4{0, 0, 0, 0};
+                    store_grad<T>(a, row, c, y);
+                }
+            }
+        }
+    }
+    finish_sums(a, sums, part);
+}
+
+template <typename T, bool GRAD>
+void launch_policy_loss(const PolicyLossArgs &a, hipStream_t s, int *blocks) {
+    // Lanes per row and 16-byte pieces per lane by the row's length (pieces of 4 f32 or 8 16-bit values)
+    const int A = a.n_actions, chunks = (A + Chunk<T>::V - 1) / Chunk<T>::V;
+    const auto grid = [&](int rows_per_block, int most) {
+        *blocks = static_cast<int>(std::min<long long>(most, (a.rows + rows_per_block - 1) / rows_per_block));
+        return dim3(*blocks);
+    };
+    if (A <= 4) oc_policy_loss_rows_kernel<T, 4, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
+    else if (A <= 8) oc_policy_loss_rows_kernel<T, 8, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
+    else if (A <= 16) oc_policy_loss_rows_kernel<T, 16, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
+    else if (chunks <= 16) oc_policy_loss_group_kernel<T, 16, 1, GRAD><<<grid(16, kMaxBlocks), 256, 0, s>>>(a);
+    else if (chunks <= 64) oc_policy_loss_group_kernel<T, 16, 4, GRAD><<<grid(16, kMaxBlocks), 256, 0, s>>>(a);
+    else if (chunks <= 64 * 4) oc_policy_loss_group_kernel<T, 64, 4, GRAD><<<grid(4, kMaxBlocks), 256, 0, s>>>(a);
+    else if (chunks <= 256 * 4) oc_policy_loss_group_kernel<T, 256, 4, GRAD><<<grid(1, kMaxBlocks), 256, 0, s>>>(a);
+    else if (chunks <= 512 * 8) oc_policy_loss_group_kernel<T, 512, 8, GRAD><<<grid(1, kMaxBlocks), 512, 0, s>>>(a);
+    else oc_policy_loss_group_kernel<T, 1024, 0, GRAD><<<grid(1, kMaxBlocks), 1024, 0, s>>>(a);
+}
+
+// Few rows: every block adds the weights up itself (8 bytes a row out of L2) and saves the launch that does it.
+constexpr long long kSelfWeightRows = 8192;
+
+template <bool GRAD>
+void launch_policy_loss_type(const PolicyLossArgs &a, int type, hipStream_t s, int *blocks) {
+    if (type == OC_F32) launch_policy_loss<float, GRAD>(a, s, blocks);
+    else if (type == OC_BF16) launch_policy_loss<__bf16, GRAD>(a, s, blocks);
+    else launch_policy_loss<_Float16, GRAD>(a, s, blocks);
+}
+
+}  // namespace
+
+extern "C" int64_t oc_policy_loss_workspace_bytes(void) {
+    return static_cast<int64_t>(kWeightBlocks + static_cast<int64_t>(kMaxBlocks) * kSums) * sizeof(double);
+}
+
+extern "C" int oc_policy_loss(const oc_policy_loss_args *p, int what, void *d_workspace, void *stream) {
+    if (!p || what < OC_LOSS_FORWARD || what > OC_LOSS_BACKWARD)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: NULL arguments or an unknown pass");
+    if (p->rows < 0 || p->n_actions < 1 || p->row_stride < p->n_actions || p->available_stride < 0)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: rows %lld, n_actions %d, row_stride %lld, available_stride %lld",
+                                static_cast<long long>(p->rows), p->n_actions, static_cast<long long>(p->row_stride), static_cast<long long>(p->available_stride));
+    if (p->logits_type < OC_F32 || p->logits_type > OC_F16 || p->action_type < OC_ACT_I32 || p->action_type > OC_ACT_F32)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: logits_type %d, action_type %d", p->logits_type, p->action_type);
+    if ((p->rows > 0 && (!p->d_logits || !p->d_actions || !p->d_old_log_probs || !p->d_advantages)) ||
+        (p->rows > 0 && what != OC_LOSS_FORWARD && !p->d_grad) || (what == OC_LOSS_BACKWARD ? !p->d_weight : !p->d_loss || !d_workspace))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: a required pointer is NULL");
+    const uintptr_t element = p->logits_type == OC_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(p->d_logits) % element || reinterpret_cast<uintptr_t>(p->d_grad) % element ||
+        reinterpret_cast<uintptr_t>(p->d_weight) % 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: a pointer is not aligned to its elements (workspace: 8 bytes)");
+    if (!(p->clip_param >= 0.0))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: clip_param %g", p->clip_param);
+    if (p->rows == 0 && what == OC_LOSS_BACKWARD) return OC_OK;
+    PolicyLossArgs a = {};
+    a.logits = p->d_logits; a.actions = p->d_actions; a.old_logp = p->d_old_log_probs; a.adv = p->d_advantages;
+    a.ref_logp = p->d_ref_log_probs; a.weights = p->d_active_masks; a.avail = p->d_available; a.grad = p->d_grad;
+    a.grad_out = what == OC_LOSS_BACKWARD ? p->d_grad_out : nullptr;
+    a.loss = p->d_loss; a.stats = p->d_stats; a.weight = p->d_weight;
+    a.weight_partials = static_cast<double *>(d_workspace);
+    a.sums = a.weight_partials + kWeightBlocks;
+    a.rows = p->rows; a.row_stride = p->row_stride; a.avail_stride = p->available_stride;
+    a.n_actions = p->n_actions; a.action_type = p->action_type; a.avail_u8 = p->available_u8 != 0;
+    a.clip_lo = static_cast<float>(1.0 - p->clip_param); a.clip_hi = static_cast<float>(1.0 + p->clip_param);
+    a.entropy_coef = p->entropy_coef; a.kl_coef = p->kl_coef; a.grad_scale = what == OC_LOSS_FORWARD ? 1.0f : p->grad_scale;
+    const OcDeviceScope on_device(oc_device_of_pointer(what == OC_LOSS_BACKWARD ? static_cast<const void *>(p->d_weight) : p->d_loss));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    a.want_sums = what != OC_LOSS_BACKWARD;
+    a.weight_from = what == OC_LOSS_FORWARD ? WEIGHT_NONE : what == OC_LOSS_BACKWARD ? WEIGHT_GIVEN : a.rows <= kSelfWeightRows ? WEIGHT_SELF : WEIGHT_PARTIALS;
+    if (a.weight_from == WEIGHT_PARTIALS) {
+        a.n_weight_partials = static_cast<int>(std::min<long long>(kWeightBlocks, (a.rows + 255) / 256));
+        oc_policy_weight_kernel<<<dim3(a.n_weight_partials), 256, 0, s>>>(a);
+    }
+    int blocks = 0;
+    // one block finishes by itself
+    const int rows_per_block = a.n_actions <= 16 ? kRowTile : 1;
+    a.finalize_here = a.rows <= rows_per_block;
+    if (a.rows == 0) {
+        oc_policy_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, 0);
+    } else {
+        if (what == OC_LOSS_FORWARD) launch_policy_loss_type<false>(a, p->logits_type, s, &blocks);
+        else launch_policy_loss_type<true>(a, p->logits_type, s, &blocks);
+        if (a.want_sums && !a.finalize_here) oc_policy_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, blocks);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_policy_loss: %s", hipGetErrorString(e));
+}
+
+// ======================================================================================================
+// Clipped value loss and its gradient (train/MAPPO/r_mappo.py, cal_value_loss): per sample with target y = (return - mean) / std
+//   e0 = y - v,  e1 = y - (v0 + clamp(v - v0, -c, c)),  loss = max(h(e0), h(e1)),  h(e) = e^2 / 2, or Huber's with delta;
+//   d loss / d v = -h'(e0) where |v - v0| <= c or h(e0) >= h(e1), else 0 (the clamped branch does not move with v).
+// 12..16 bytes read and 4 written per sample, nothing used twice: four samples per lane in one load each.
+// ======================================================================================================
+namespace {
+
+struct ValueLossArgs {
+    const void *values;
+    const float *preds, *returns, *weights;
+    void *grad;
+    const float *grad_out;
+    float *loss;
+    double *weight;
+    double *weight_partials, *sums;                        // [kWeightBlocks], [blocks][2]
+    long long n;
+    float clip, delta, mean, std, grad_scale;              // clip < 0: not clipped; delta < 0: e^2 / 2
+    int weight_from, n_weight_partials, finalize_here, want_sums;
+};
+
+__global__ __launch_bounds__(256) void oc_value_weight_kernel(const ValueLossArgs a) {
+    __shared__ double part[4];
+    double w = 0.0;
+    const long long stride = static_cast<long long>(gridDim.x) * 256, n4 = a.n >> 2;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n4; i += stride) {
+        const u32x4 q = reinterpret_cast<const u32x4_a4 *>(a.weights)[i];
+        w += (static_cast<double>(__uint_as_float(q[0])) + __uint_as_float(q[1])) + (static_cast<double>(__uint_as_float(q[2])) + __uint_as_float(q[3]));
+    }
+    if (blockIdx.x == 0 && threadIdx.x < (a.n & 3)) w += a.weights[(n4 << 2) + threadIdx.x];
+    w = block_sum(w, part);
+    if (threadIdx.x == 0) a.weight_partials[blockIdx.x] = w;
+}
+
+__device__ __forceinline__ float value_sample(const ValueLossArgs &a, float v, float v0, float ret, float w, float scale, double &sum) {
+    if (w == 0.0f) return 0.0f;
+    const float y = (ret - a.mean) / a.std;
+    const float e0 = y - v, step = v - v0;
+    float h0, h1, slope;
+    bool free_ = true;
+    if (a.delta >= 0.0f) {
+        h0 = fabsf(e0) <= a.delta ? 0.5f * e0 * e0 : a.delta * (fabsf(e0) - 0.5f * a.delta);
+        slope = e0 > a.delta ? a.delta : e0 < -a.delta ? -a.delta : e0;       // a NaN stays
+    } else {
+        h0 = 0.5f * e0 * e0;
+        slope = e0;
+    }
+    float worst = h0;
+    if (a.clip >= 0.0f && fabsf(step) > a.clip) {
+        const float e1 = y - (v0 + copysignf(a.clip, step));
+        h1 = a.delta >= 0.0f && fabsf(e1) > a.delta ? a.delta * (fabsf(e1) - 0.5f * a.delta) : 0.5f * e1 * e1;
+        free_ = !(h0 < h1);
+        worst = free_ ? h0 : h1;
+    }
+    sum += static_cast<double>(w) * static_cast<double>(worst);
+    return free_ ? -scale * w * slope : 0.0f;
+}
+
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void oc_value_loss_kernel(const ValueLossArgs a) {
+    __shared__ double part[4];
+    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    float scale = 0.0f;
+    if (GRAD) {
+        double w = 0.0;
+        if (!a.weights) {
+            w = static_cast<double>(a.n);
+        } else if (a.weight_from == WEIGHT_SELF) {
+            for (long long i = threadIdx.x; i < a.n; i += 256) w += a.weights[i];
+            w = block_sum(w, part);
+        } else if (a.weight_from == WEIGHT_PARTIALS) {
+            for (int i = threadIdx.x; i < a.n_weight_partials; i += 256) w += a.weight_partials[i];
+            w = block_sum(w, part);
+        } else {
+            w = *a.weight;
+        }
+        scale = w != 0.0 ? static_cast<float>(1.0 / w) * a.grad_scale * (a.grad_out ? *a.grad_out : 1.0f) : 0.0f;
+    }
+    double sum = 0.0, weight = 0.0;
+    const long long n4 = a.n >> 2, stride = static_cast<long long>(gridDim.x) * 256;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n4; i += stride) {
+        const four_t v = reinterpret_cast<const four_t *>(a.values)[i];
+        const u32x4 v0 = reinterpret_cast<const u32x4_a4 *>(a.preds)[i], ret = reinterpret_cast<const u32x4_a4 *>(a.returns)[i];
+        u32x4 w4 = {0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u};
+        if (a.weights) w4 = reinterpret_cast<const u32x4_a4 *>(a.weights)[i];
+        four_t g;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = __uint_as_float(w4[k]);
+            weight += static_cast<double>(w);
+            g[k] = static_cast<T>(value_sample(a, static_cast<float>(v[k]), __uint_as_float(v0[k]), __uint_as_float(ret[k]), w, scale, sum));
+        }
+        if (GRAD) reinterpret_cast<four_t *>(a.grad)[i] = g;
+    }
+    if (blockIdx.x == 0 && threadIdx.x < (a.n & 3)) {
+        const long long i = (n4 << 2) + threadIdx.x;
+        const float w = a.weights ? a.weights[i] : 1.0f;
+        weight += static_cast<double>(w);
+        const float g = value_sample(a, static_cast<float>(static_cast<const T *>(a.values)[i]), a.preds[i], a.returns[i], w, scale, sum);
+        if (GRAD) static_cast<T *>(a.grad)[i] = static_cast<T>(g);
+    }
+    if (!a.want_sums) return;
+    sum = block_sum(sum, part);
+    weight = block_sum(weight, part);
+    if (threadIdx.x != 0) return;
+    if (a.finalize_here) {
+        *a.loss = static_cast<float>(weight != 0.0 ? sum / weight : 0.0);
+        if (a.weight) *a.weight = weight;
+    } else {
+        a.sums[2 * blockIdx.x] = sum;
+        a.sums[2 * blockIdx.x + 1] = weight;
+    }
+}
+
+__global__ __launch_bounds__(256) void oc_value_finalize_kernel(const ValueLossArgs a, int blocks) {
+    __shared__ double part[4];
+    double sum = 0.0, weight = 0.0;
+    for (int b = threadIdx.x; b < blocks; b += 256) {
+        sum += a.sums[2 * b];
+        weight += a.sums[2 * b + 1];
+    }
+    sum = block_sum(sum, part);
+    weight = block_sum(weight, part);
+    if (threadIdx.x == 0) {
+        *a.loss = static_cast<float>(weight != 0.0 ? sum / weight : 0.0);
+        if (a.weight) *a.weight = weight;
+    }
+}
+
+template <typename T>
+void launch_value_loss(const ValueLossArgs &a, int grad, int blocks, hipStream_t s) {
+    if (grad) oc_value_loss_kernel<T, true><<<dim3(blocks), 256, 0, s>>>(a);
+    else oc_value_loss_kernel<T, false><<<dim3(blocks), 256, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" int64_t oc_value_loss_workspace_bytes(void) { return static_cast<int64_t>(kWeightBlocks + 2 * kMaxBlocks) * sizeof(double); }
+
+extern "C" int oc_value_loss(const oc_value_loss_args *p, int what, void *d_workspace, void *stream) {
+    if (!p || what < OC_LOSS_FORWARD || what > OC_LOSS_BACKWARD)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: NULL arguments or an unknown pass");
+    if (p->n < 0 || p->values_type < OC_F32 || p->values_type > OC_F16)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: n %lld, values_type %d", static_cast<long long>(p->n), p->values_type);
+    if ((p->n > 0 && (!p->d_values || !p->d_value_preds || !p->d_returns)) || (p->n > 0 && what != OC_LOSS_FORWARD && !p->d_grad) ||
+        (what == OC_LOSS_BACKWARD ? !p->d_weight : !p->d_loss || !d_workspace))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: a required pointer is NULL");
+    const uintptr_t element = p->values_type == OC_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(p->d_values) % element || reinterpret_cast<uintptr_t>(p->d_grad) % element ||
+        reinterpret_cast<uintptr_t>(p->d_weight) % 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: a pointer is not aligned to its elements (workspace: 8 bytes)");
+    if (p->n == 0 && what == OC_LOSS_BACKWARD) return OC_OK;
+    ValueLossArgs a = {};
+    a.values = p->d_values; a.preds = p->d_value_preds; a.returns = p->d_returns; a.weights = p->d_active_masks;
+    a.grad = p->d_grad; a.grad_out = what == OC_LOSS_BACKWARD ? p->d_grad_out : nullptr; a.loss = p->d_loss; a.weight = p->d_weight;
+    a.weight_partials = static_cast<double *>(d_workspace);
+    a.sums = a.weight_partials + kWeightBlocks;
+    a.n = p->n;
+    a.clip = p->clip_param; a.delta = p->huber_delta; a.mean = p->mean; a.std = p->std;
+    a.grad_scale = what == OC_LOSS_FORWARD ? 1.0f : p->grad_scale;
+    a.want_sums = what != OC_LOSS_BACKWARD;
+    const OcDeviceScope on_device(oc_device_of_pointer(what == OC_LOSS_BACKWARD ? static_cast<const void *>(p->d_weight) : p->d_loss));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    a.weight_from = what == OC_LOSS_FORWARD ? WEIGHT_NONE : what == OC_LOSS_BACKWARD ? WEIGHT_GIVEN : a.n <= kSelfWeightRows ? WEIGHT_SELF : WEIGHT_PARTIALS;
+    if (a.weight_from == WEIGHT_PARTIALS && a.weights) {
+        a.n_weight_partials = static_cast<int>(std::min<long long>(kWeightBlocks, (a.n + 1023) / 1024));
+        oc_value_weight_kernel<<<dim3(a.n_weight_partials), 256, 0, s>>>(a);
+    }
+    const int blocks = static_cast<int>(std::min<long long>(kMaxBlocks, (a.n + 1023) / 1024));
+    a.finalize_here = blocks == 1;
+    if (a.n == 0) {
+        oc_value_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, 0);
+    } else {
+        if (p->values_type == OC_F32) launch_value_loss<float>(a, what != OC_LOSS_FORWARD, blocks, s);
+        else if (p->values_type == OC_BF16) launch_value_loss<__bf16>(a, what != OC_LOSS_FORWARD, blocks, s);
+        else launch_value_loss<_Float16>(a, what != OC_LOSS_FORWARD, blocks, s);
+        if (a.want_sums && !a.finalize_here) oc_value_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, blocks);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_value_loss: %s", hipGetErrorString(e));
+}
+
+// ======================================================================================================
+// Global norm of many gradient tensors and clipping (train/MAPPO/r_mappo.py clips each network's gradients with
+// torch.nn.utils.clip_grad_norm_; get_gard_norm of utils/util.py is the norm alone):
+//   norm = sqrt(sum g^2) over all elements of all tensors, or max |g|;  g <- g * min(1, max_norm / (norm + 1e-6)).
+// Two passes, because the factor needs every element: read all, then read and write all.  The tensors' addresses travel in the kernel
+// arguments (no table to copy, nothing kept between calls), kTensors at a time.  The squares are added in f64: neither 1e-30 nor 1e30
+// leaves the range, and the order of the sums does not show.  The second pass adds up the first one's partial sums in every block.
+// ======================================================================================================
+namespace {
+
+constexpr int kTensors = 120;                              // kernel arguments stay below 4 KB
+constexpr int kNormBlocks = 2048;                          // pieces that the elements are cut into, beside one per tensor
+constexpr long long kPiece = 4096;                         // and their unit
+
+struct NormArgs {
+    const void *src[kTensors];
+    void *dst[kTensors];
+    long long numel[kTensors];
+    int first_block[kTensors + 1];                         // of this launch
+    uint8_t type[kTensors];
+    long long piece;
+    double *partials;                                      // of the whole call
+    float *norm;
+    float max_norm;
+    int n, block0, n_partials, inf_norm, write_norm, in_place;
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ int tensor_of_block(const NormArgs &a, int block) {
+    int lo = 0, hi = a.n;                                  // first_block[lo] <= block < first_block[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.first_block[mid] <= block) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double join(double x, double y, int inf_norm) {
+    if (!inf_norm) return x + y;
+    return x != x || y != y ? x + y : fmax(x, y);           // a NaN stays
+}
+
+__device__ __forceinline__ double block_join(double x, int inf_norm, double *part) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x = join(x, __shfl_xor(x, off), inf_norm);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return join(join(part[0], part[1], inf_norm), join(part[2], part[3], inf_norm), inf_norm);
+}
+
+template <typename T>
+__device__ __forceinline__ double norm_of_piece(const T *p, long long n, int inf_norm) {
+    constexpr int V = 16 / sizeof(T);
+    typedef typename Unaligned<sizeof(T)>::type U;
+    double sum[4] = {0, 0, 0, 0};
+    const long long chunks = n / V;
+    const auto take = [&](const Chunk<T> &c) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float f = static_cast<float>(c.e[k]);
+            if (inf_norm) {
+                sum[k & 3] = join(sum[k & 3], static_cast<double>(fabsf(f)), 1);
+            } else {
+                const double d = static_cast<double>(f);
+                sum[k & 3] = fma(d, d, sum[k & 3]);
+            }
+        }
+    };
+    long long i = threadIdx.x;
+    for (; i + 768 < chunks; i += 1024) {                  // four loads in flight
+        Chunk<T> c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) c[u].raw = reinterpret_cast<const U *>(p)[i + 256 * u];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) take(c[u]);
+    }
+    for (; i < chunks; i += 256) {
+        Chunk<T> c;
+        c.raw = reinterpret_cast<const U *>(p)[i];
+        take(c);
+    }
+    for (long long j = chunks * V + threadIdx.x; j < n; j += 256) {
+        const double d = static_cast<double>(static_cast<float>(p[j]));
+        sum[0] = inf_norm ? join(sum[0], fabs(d), 1) : fma(d, d, sum[0]);
+    }
+    return join(join(sum[0], sum[1], inf_norm), join(sum[2], sum[3], inf_norm), inf_norm);
+}
+
+__global__ __launch_bounds__(256) void oc_grad_norm_kernel(const NormArgs a) {
+    __shared__ double part[4];
+    const int t = tensor_of_block(a, blockIdx.x);
+    const long long from = (static_cast<long long>(blockIdx.x) - a.first_block[t]) * a.piece;
+    const long long n = a.numel[t] - from < a.piece ? a.numel[t] - from : a.piece;
+    double x = 0.0;
+    if (n > 0) {
+        if (a.type[t] == OC_F32) x = norm_of_piece(static_cast<const float *>(a.src[t]) + from, n, a.inf_norm);
+        else if (a.type[t] == OC_BF16) x = norm_of_piece(static_cast<const __bf16 *>(a.src[t]) + from, n, a.inf_norm);
+        else x = norm_of_piece(static_cast<const _Float16 *>(a.src[t]) + from, n, a.inf_norm);
+    }
+    x = block_join(x, a.inf_norm, part);
+    if (threadIdx.x == 0) a.partials[a.block0 + blockIdx.x] = x;
+}
+
+__device__ __forceinline__ float total_norm(const NormArgs &a, double *part) {
+    double x = 0.0;
+    for (int i = threadIdx.x; i < a.n_partials; i += 256) x = join(x, a.partials[i], a.inf_norm);
+    x = block_join(x, a.inf_norm, part);
+    return static_cast<float>(a.inf_norm ? x : sqrt(x));
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_piece(const T *src, T *dst, long long n, float f) {
+    constexpr int V = 16 / sizeof(T);
+    typedef typename Unaligned<sizeof(T)>::type U;
+    const long long chunks = n / V;
+    const auto scaled = [&](Chunk<T> c) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) c.e[k] = static_cast<T>(static_cast<float>(c.e[k]) * f);
+        return c.raw;
+    };
+    long long i = threadIdx.x;
+    for (; i + 768 < chunks; i += 1024) {
+        Chunk<T> c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) c[u].raw = reinterpret_cast<const U *>(src)[i + 256 * u];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) reinterpret_cast<U *>(dst)[i + 256 * u] = scaled(c[u]);
+    }
+    for (; i < chunks; i += 256) {
+        Chunk<T> c;
+        c.raw = reinterpret_cast<const U *>(src)[i];
+        reinterpret_cast<U *>(dst)[i] = scaled(c);
+    }
+    for (long long j = chunks * V + threadIdx.x; j < n; j += 256) dst[j] = static_cast<T>(static_cast<float>(src[j]) * f);
+}
+
+__global__ __launch_bounds__(256) void oc_grad_clip_kernel(const NormArgs a) {
+    __shared__ double part[4];
+    const float norm = total_norm(a, part);
+    if (a.write_norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    if (a.max_norm < 0.0f || a.n == 0) return;             // the norm alone, or no element at all
+    const float factor = a.max_norm / (norm + 1e-6f);
+    const float f = factor > 1.0f ? 1.0f : factor;         // a NaN norm makes every gradient NaN, as the product does
+    if (a.in_place && f == 1.0f) return;                   // nothing to clip: the gradients stay as they are
+    const int t = tensor_of_block(a, blockIdx.x);
+    const long long from = (static_cast<long long>(blockIdx.x) - a.first_block[t]) * a.piece;
+    const long long n = a.numel[t] - from < a.piece ? a.numel[t] - from : a.piece;
+    if (n <= 0) return;
+    if (a.type[t] == OC_F32) scale_piece(static_cast<const float *>(a.src[t]) + from, static_cast<float *>(a.dst[t]) + from, n, f);
+    else if (a.type[t] == OC_BF16) scale_piece(static_cast<const __bf16 *>(a.src[t]) + from, static_cast<__bf16 *>(a.dst[t]) + from, n, f);
+    else scale_piece(static_cast<const _Float16 *>(a.src[t]) + from, static_cast<_Float16 *>(a.dst[t]) + from, n, f);
+}
+
+}  // namespace
+
+extern "C" int64_t oc_grad_norm_workspace_bytes(int32_t n_tensors) {
+    return n_tensors < 0 ? -1 : (static_cast<int64_t>(kNormBlocks) + n_tensors) * static_cast<int64_t>(sizeof(double));
+}
+
+extern "C" int oc_grad_norm_clip(int32_t n_tensors, const void *const *d_grads, void *const *d_out, const int64_t *numel, const int32_t *types,
+                                 float max_norm, int inf_norm, float *d_norm, void *d_workspace, void *stream) {
+    if (n_tensors < 0 || !d_norm || !d_workspace || (n_tensors > 0 && (!d_grads || !numel || !types)))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grad_norm_clip: n_tensors %d or a required pointer is NULL", n_tensors);
+    if (reinterpret_cast<uintptr_t>(d_workspace) % 8 || max_norm != max_norm)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grad_norm_clip: workspace not aligned to 8 bytes, or max_norm is NaN");
+    long long total = 0;
+    for (int i = 0; i < n_tensors; ++i) {
+        if (numel[i] < 0 || types[i] < OC_F32 || types[i] > OC_F16)
+            return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grad_norm_clip: tensor %d has %lld elements of type %d", i, static_cast<long long>(numel[i]), types[i]);
+        const uintptr_t element = types[i] == OC_F32 ? 4 : 2;
+        const uintptr_t src = reinterpret_cast<uintptr_t>(d_grads[i]), dst = d_out ? reinterpret_cast<uintptr_t>(d_out[i]) : src;
+        if (numel[i] > 0 && (!src || !dst || src % element || dst % element))
+            return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grad_norm_clip: tensor %d is NULL or not aligned to its elements", i);
+        total += numel[i];
+    }
+    // pieces of one size: at most kNormBlocks of them, and one more per tensor for its rest
+    const long long piece = std::max<long long>(kPiece, ((total + kNormBlocks - 1) / kNormBlocks + kPiece - 1) / kPiece * kPiece);
+    const OcDeviceScope on_device(oc_device_of_pointer(d_norm));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    long long n_partials = 0;
+    for (int i = 0; i < n_tensors; ++i) n_partials += (numel[i] + piece - 1) / piece;
+    for (int pass = 0; pass < 2; ++pass) {
+        int block0 = 0, i = 0;
+        bool first = true;
+        do {
+            NormArgs a;
+            a.n = 0;
+            a.piece = piece; a.partials = static_cast<double *>(d_workspace); a.norm = d_norm; a.max_norm = max_norm;
+            a.block0 = block0; a.n_partials = static_cast<int>(n_partials); a.inf_norm = inf_norm != 0; a.write_norm = first; a.in_place = d_out == nullptr;
+            int blocks = 0;
+            for (; i < n_tensors && a.n < kTensors; ++i) {
+                if (numel[i] == 0) continue;
+                a.src[a.n] = d_grads[i];
+                a.dst[a.n] = d_out ? d_out[i] : const_cast<void *>(d_grads[i]);
+                a.numel[a.n] = numel[i];
+                a.type[a.n] = static_cast<uint8_t>(types[i]);
+                a.first_block[a.n++] = blocks;
+                blocks += static_cast<int>((numel[i] + piece - 1) / piece);
+            }
+            a.first_block[a.n] = blocks;
+            if (pass == 0) {
+                if (blocks) oc_grad_norm_kernel<<<dim3(blocks), 256, 0, s>>>(a);
+            } else if (first || (blocks && max_norm >= 0.0f)) {
+                // without a clip, and without any element, one block writes the norm
+                oc_grad_clip_kernel<<<dim3(blocks && max_norm >= 0.0f ? blocks : 1), 256, 0, s>>>(a);
+            }
+            block0 += blocks;
+            first = false;
+        } while (i < n_tensors);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grad_norm_clip: %s", hipGetErrorString(e));
+}

@@ -24,7 +24,7 @@ DIAGNOSTICS = os.environ.get("OC_DIAGNOSTICS", "0") not in ("", "0")
 LIB_OVERRIDE = os.environ.get("OC_LIB_PATH", "")
 LIB_PATH = LIB_OVERRIDE or os.path.join(CSRC, "liboc_hip_asan.so" if SANITIZE else "liboc_hip_diag.so" if DIAGNOSTICS else "liboc_hip.so")
 SOURCES = [os.path.join(CSRC, "overcooked_engine.hip"), os.path.join(CSRC, "rollout_ops.hip"),
-           os.path.join(CSRC, "policy_ops.hip")]
+           os.path.join(CSRC, "policy_ops.hip"), os.path.join(CSRC, "update_ops.hip")]
 HEADERS = [os.path.join(CSRC, "policy_pack.h"), os.path.join(CSRC, "oc_internal.h"), os.path.join(CSRC, "policy_block_body.h"), os.path.join(CSRC, "policy_mono_loop.h"),
            os.path.join(CSRC, "policy_duo_kernel.h"), os.path.join(CSRC, "policy_duo_body.h"),
            os.path.join(CSRC, "oc_np_kernels.h")]
@@ -56,6 +56,7 @@ SYMBOLS_ENV = [
 # ... include/overcooked_ops.h -- policy inference, rollouts with the policies in the loop, GAE, minibatch gathers
 SYMBOLS_OPS = [
     "oc_gae_returns", "oc_advantage_workspace_bytes", "oc_advantage_normalize", "oc_gather_rows", "oc_gather_columns", "oc_pack_columns", "oc_gather_records",
+    "oc_policy_loss_workspace_bytes", "oc_policy_loss", "oc_value_loss_workspace_bytes", "oc_value_loss", "oc_grad_norm_workspace_bytes", "oc_grad_norm_clip",
     "oc_policy_packed_bytes", "oc_policy_pack_host", "oc_policy_pack", "oc_policy_plan_tiles", "oc_policy_forward", "oc_policy_forward_multi",
     "oc_policy_plan_tiles_multi", "oc_group_policy_rollout_multi", "oc_policy_uniform", "oc_policy_rollout", "oc_group_policy_rollout",
     "oc_partition_rows", "oc_policy_forward_gather", "oc_policy_rollout_mixed",
@@ -88,6 +89,24 @@ class OcPolicyMultiSlot(ctypes.Structure):
     _fields_ = [("shape", ctypes.POINTER(OcPolicyShape)), ("d_packed", ctypes.c_void_p), ("n_nets", ctypes.c_int32),
                 ("d_obs", ctypes.c_void_p), ("n_rows", ctypes.c_int64), ("d_raw", ctypes.c_void_p), ("d_actions", ctypes.c_void_p),
                 ("d_action_logp", ctypes.c_void_p), ("d_logp", ctypes.c_void_p), ("d_row_select", ctypes.c_void_p), ("seed", ctypes.c_uint32)]
+
+
+class OcPolicyLossArgs(ctypes.Structure):
+    """oc_policy_loss_args"""
+    _fields_ = [("d_logits", ctypes.c_void_p), ("d_actions", ctypes.c_void_p), ("d_old_log_probs", ctypes.c_void_p), ("d_advantages", ctypes.c_void_p),
+                ("d_ref_log_probs", ctypes.c_void_p), ("d_active_masks", ctypes.c_void_p), ("d_available", ctypes.c_void_p), ("d_loss", ctypes.c_void_p),
+                ("d_stats", ctypes.c_void_p), ("d_weight", ctypes.c_void_p), ("d_grad", ctypes.c_void_p), ("d_grad_out", ctypes.c_void_p), ("rows", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("available_stride", ctypes.c_int64), ("n_actions", ctypes.c_int32), ("logits_type", ctypes.c_int32), ("action_type", ctypes.c_int32),
+                ("available_u8", ctypes.c_int32), ("clip_param", ctypes.c_double), ("entropy_coef", ctypes.c_float), ("kl_coef", ctypes.c_float),
+                ("grad_scale", ctypes.c_float)]
+
+
+class OcValueLossArgs(ctypes.Structure):
+    """oc_value_loss_args"""
+    _fields_ = [("d_values", ctypes.c_void_p), ("d_value_preds", ctypes.c_void_p), ("d_returns", ctypes.c_void_p), ("d_active_masks", ctypes.c_void_p),
+                ("d_loss", ctypes.c_void_p), ("d_weight", ctypes.c_void_p), ("d_grad", ctypes.c_void_p), ("d_grad_out", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("values_type", ctypes.c_int32), ("clip_param", ctypes.c_float), ("huber_delta", ctypes.c_float), ("mean", ctypes.c_float),
+                ("std", ctypes.c_float), ("grad_scale", ctypes.c_float)]
 
 
 class OcLayoutParams(ctypes.Structure):
@@ -220,6 +239,15 @@ def lib():
                                     ctypes.POINTER(vp), ctypes.POINTER(vp), vp, i64, i64, i64, vp]
     L.oc_pack_columns.argtypes = [ctypes.c_int32, ctypes.POINTER(vp), i64, vp, vp]
     L.oc_gather_records.argtypes = [vp, i64, ctypes.c_int32, ctypes.POINTER(vp), ctypes.c_int32, vp, vp, i64, i64, i64, vp]
+    L.oc_policy_loss_workspace_bytes.argtypes = []
+    L.oc_policy_loss_workspace_bytes.restype = i64
+    L.oc_policy_loss.argtypes = [ctypes.POINTER(OcPolicyLossArgs), i32, vp, vp]
+    L.oc_value_loss_workspace_bytes.argtypes = []
+    L.oc_value_loss_workspace_bytes.restype = i64
+    L.oc_value_loss.argtypes = [ctypes.POINTER(OcValueLossArgs), i32, vp, vp]
+    L.oc_grad_norm_workspace_bytes.argtypes = [ctypes.c_int32]
+    L.oc_grad_norm_workspace_bytes.restype = i64
+    L.oc_grad_norm_clip.argtypes = [ctypes.c_int32, vp, vp, vp, vp, fp, i32, vp, vp, vp]
     ps = ctypes.POINTER(OcPolicyShape)
     L.oc_policy_packed_bytes.argtypes = [ps]
     L.oc_policy_packed_bytes.restype = i64

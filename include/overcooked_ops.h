@@ -64,6 +64,76 @@ int oc_gather_records(const void *d_packed, int64_t src_rows, int32_t n_cols, vo
                       const float *d_norm_stats, const int64_t *d_index, int64_t n_rows, int64_t row_mul, int64_t row_add,
                       void *stream);
 
+/* ---- the update: losses with their gradients, gradient clipping ------------------------------------------------
+ * Element types of the tensors below. */
+enum { OC_F32 = 0, OC_BF16 = 1, OC_F16 = 2 };
+#define OC_ACT_F32 2           /* actions stored as floats (the reference's buffers), beside OC_ACT_I32 / OC_ACT_I64 */
+/* The pass of a loss: value only; value and gradient in one go; the gradient after a forward pass (autograd). */
+enum { OC_LOSS_FORWARD = 0, OC_LOSS_FORWARD_GRAD = 1, OC_LOSS_BACKWARD = 2 };
+
+/* Clipped policy loss over logits with an entropy bonus and a KL term to a reference policy, and its gradient: the arithmetic of
+ * R_MAPPO.ppo_update's policy half (train/MAPPO/r_mappo.py: imp_weights, surr1, surr2, active_masks) behind
+ * FixedCategorical(logits) with unavailable actions taken out (train/MAPPO/utils/distributions.py).  Per row r with taken action a:
+ *   action j is possible when it is available and logit j is not -inf;   lp = z_a - log sum_{possible j} exp z_j
+ *   ratio = exp(lp - old);  H = -sum p log p;  kl = exp(ref - lp) - (ref - lp) - 1
+ *   loss = 1/W sum_r w ( -min(ratio A, clamp(ratio, 1-c, 1+c) A) - entropy_coef H + kl_coef kl )
+ * W is the sum of the active masks over the rows whose action lies in [0, n_actions); an action outside marks padding.  A row of weight 0
+ * is not read; a row without a possible action, or whose taken action is not possible, adds nothing and gets a gradient of 0.  W == 0
+ * gives a loss of 0.  Logits of impossible actions may hold anything and get a gradient of 0; a NaN or +inf of a possible action makes
+ * the loss and the row's gradient NaN.
+ * d_loss: one f32; d_stats (f32[5] or NULL): the means of the clipped term, the entropy, kl, the share of clipped ratios, the ratio;
+ * d_weight (NULL unless a backward pass follows): W.  BACKWARD reads W from there (the same inputs' forward pass) and multiplies by
+ * *d_grad_out (device; NULL = 1).  The gradient is contiguous [rows][n_actions], times grad_scale, and may not overlap the logits.  d_workspace: oc_policy_loss_workspace_bytes() bytes, 8-byte
+ * aligned, needed by the two forward passes, free for other use when they are through. */
+typedef struct {
+    const void *d_logits;              /* [rows] of n_actions values, row_stride elements apart */
+    const void *d_actions;             /* [rows], see action_type */
+    const float *d_old_log_probs, *d_advantages;
+    const float *d_ref_log_probs;      /* NULL: no KL term */
+    const float *d_active_masks;       /* NULL: all 1 */
+    const void *d_available;           /* NULL: all; else [rows] of n_actions f32 or bytes, non-zero = available, available_stride elements apart (0: one row for all) */
+    float *d_loss, *d_stats;
+    double *d_weight;
+    void *d_grad;
+    const float *d_grad_out;
+    int64_t rows, row_stride, available_stride;
+    int32_t n_actions, logits_type, action_type, available_u8;
+    double clip_param;
+    float entropy_coef, kl_coef, grad_scale;
+} oc_policy_loss_args;
+int64_t oc_policy_loss_workspace_bytes(void);
+int oc_policy_loss(const oc_policy_loss_args *args, int what, void *d_workspace, void *stream);
+
+/* Clipped value loss and its gradient (R_MAPPO.cal_value_loss, train/MAPPO/r_mappo.py; huber_loss / mse_loss of train/MAPPO/utils/util.py):
+ *   y = (return - mean) / std;  e0 = y - v;  e1 = y - (v0 + clamp(v - v0, -c, c));  loss = sum w max(h(e0), h(e1)) / sum w
+ * with h Huber's of huber_delta (< 0: e^2 / 2); clip_param < 0: h(e0) alone.  The gradient is that of h(e0) where |v - v0| <= c or
+ * h(e0) >= h(e1), else 0.  Samples of weight 0 are left out whatever they hold; no weight at all gives a loss of 0.
+ * Passes, d_loss, d_weight (the sum of w), grad_scale and workspace as oc_policy_loss. */
+typedef struct {
+    const void *d_values;
+    const float *d_value_preds, *d_returns;
+    const float *d_active_masks;       /* NULL: all 1 */
+    float *d_loss;
+    double *d_weight;
+    void *d_grad;
+    const float *d_grad_out;
+    int64_t n;
+    int32_t values_type;
+    float clip_param, huber_delta, mean, std, grad_scale;
+} oc_value_loss_args;
+int64_t oc_value_loss_workspace_bytes(void);
+int oc_value_loss(const oc_value_loss_args *args, int what, void *d_workspace, void *stream);
+
+/* Norm of all elements of n_tensors gradient tensors (HOST arrays of device pointers, element counts and types, each tensor one piece of
+ * memory) and clipping: norm = sqrt(sum g^2), or max |g| with inf_norm; g <- g min(1, max_norm / (norm + 1e-6)), in place or into d_out
+ * (same counts and types).  What torch.nn.utils.clip_grad_norm_ does before every optimiser step of train/MAPPO/r_mappo.py.
+ * max_norm < 0: the norm alone.  d_norm: one f32.  d_workspace: oc_grad_norm_workspace_bytes(n_tensors) bytes, 8-byte aligned.
+ * Squares are added in f64.  Gradients that need no clipping are not written in place.  A norm that is not finite scales as the formula
+ * says (NaN everywhere, or 0 and NaN). */
+int64_t oc_grad_norm_workspace_bytes(int32_t n_tensors);
+int oc_grad_norm_clip(int32_t n_tensors, const void *const *d_grads, void *const *d_out, const int64_t *numel, const int32_t *types,
+                      float max_norm, int inf_norm, float *d_norm, void *d_workspace, void *stream);
+
 /* ---- fused policy inference on the matrix cores --------------------------------------------
  * One launch evaluates every (row range, network) tile of a rollout step -- all conventions' actors and critics,
  * both sides, every pairing segment -- reading the int8 observations oc_step wrote and writing the int32 actions
