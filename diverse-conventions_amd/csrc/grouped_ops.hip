@@ -1,0 +1,552 @@
+// grouped_ops.hip -- linear layers of several networks over one batch whose rows are sorted by network (gfx950): the products of training
+// that oc_policy_forward's tables do for inference, with the gradients.
+//   forward   Y[m, n]      = sum_k X[m, k] W_g[n, k] + b_g[n]          for the rows m of group g
+//   backward  dX[m, k]     = sum_n dY[m, n] W_g[n, k]
+//             dW_g[n, k]   = sum_{m in g} dY[m, n] X[m, k],   db_g[n] = sum_{m in g} dY[m, n]
+//
+// One tile kernel does all three: out[j][i] = sum_r I(i, r) J(j, r), i along the output's contiguous dimension.  An operand is either
+// contiguous along the reduction (W and X of the forward pass) or along its own index (W for dX, both operands of dW); the tile is
+// staged in LDS as it lies in memory, and the second kind is transposed on the way to the registers (ds_read_b64_tr_b16; f32: four
+// 4-byte reads).  The matrix instruction's first operand is I, so that a lane ends up with four consecutive elements of an output row.
+//
+// Which rows belong to which group is read from the offsets on the device: a workgroup counts the row tiles of all groups, finds its
+// own, and leaves if there is none, so that ragged groups cost no host round trip and no tile crosses a group.  Tiles are dealt to the
+// eight XCDs in contiguous runs: workgroups that share a network's weights share an L2.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "overcooked_ops.h"
+#include "oc_internal.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+struct GroupedArgs {
+    const void *I, *J;                                     // operand of the output's contiguous index, operand of its rows
+    const void *bias;                                      // forward: [groups][ni] or NULL
+    void *out;                                             // in the operands' type, or f32 partial sums of a split reduction
+    const void *offsets;                                   // [groups + 1] int32 or int64
+    long long ld_i, ld_j, ld_out;                          // row lengths in memory, in elements
+    long long rows;                                        // of the whole batch
+    int groups, ni, nj, red;                               // ni: output row length; rows product: red; dW: nj = output rows per group
+    int offsets64, splits;
+};
+
+__device__ __forceinline__ long long offset_at(const GroupedArgs &a, int g) {
+    const long long o = a.offsets64 ? static_cast<const long long *>(a.offsets)[g] : static_cast<long long>(static_cast<const int *>(a.offsets)[g]);
+    return o < 0 ? 0 : o > a.rows ? a.rows : o;            // never outside the batch, whatever the offsets say
+}
+
+template <typename T> struct Mat;
+template <> struct Mat<__bf16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ void mma(f32x4 &c, const frag &a, const frag &b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<_Float16> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ void mma(f32x4 &c, const frag &a, const frag &b) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<float> {
+    typedef f32x4 frag;
+    static __device__ __forceinline__ void mma(f32x4 &c, const frag &a, const frag &b) {
+        // element s of the lanes' pieces is one step of four reduction indices: which ones does not matter as long as both operands agree
+#pragma unroll
+        for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    }
+};
+
+// Place of 16-byte piece c of row r of a staged tile, in bytes.  Contiguous along the reduction: rows of 128 bytes, read by 16 lanes at 16
+// different rows at once.  Otherwise: rows of N elements, read at four rows 8 apart (16-bit: and four neighbours of each).  The exclusive
+// or spreads those over the banks.
+template <typename T, bool TR, int N>
+__device__ __forceinline__ int place(int r, int c) {
+    if (!TR) return r * 128 + ((c ^ (r & 7)) << 4);
+    constexpr int kPieces = N * static_cast<int>(sizeof(T)) / 16;
+    if (sizeof(T) == 2) {
+        constexpr int kSegs = kPieces / 2;
+        const int h = ((r & 3) | (((r >> 3) & 3) << 2)) & (kSegs - 1);
+        return r * (kPieces * 16) + ((((c >> 1) ^ h) << 1 | (c & 1)) << 4);
+    }
+    return r * (kPieces * 16) + ((c ^ ((((r >> 2) & 3) << 2) & (kPieces - 1))) << 4);
+}
+
+// A tile of one operand on its way from memory to LDS: every thread carries kPer pieces of 16 bytes.
+template <typename T, bool TR, int N, int THREADS, bool VEC>
+struct Stage {
+    static constexpr int V = 16 / sizeof(T), BK = 128 / sizeof(T);
+    static constexpr int kRowPieces = TR ? N / V : 8;
+    static constexpr int kPer = N * 8 / THREADS;
+    static_assert(N * 8 % THREADS == 0, "every thread carries the same number of pieces");
+    const T *src[kPer];
+    u32x4 x[kPer];
+
+    // `at`: index of the tile's first own index, `end`: their number; r0: first reduction index
+    __device__ __forceinline__ void init(const T *base, long long ld, long long at, long long r0) {
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int q = threadIdx.x + n * THREADS, row = q / kRowPieces, c = q % kRowPieces;
+            src[n] = TR ? base + (r0 + row) * ld + at + c * V : base + (at + row) * ld + r0 + c * V;
+        }
+    }
+    // own: own indexes left from the tile's first, red: reduction indexes left from this step's first.  Outside: zeros.
+    __device__ __forceinline__ void load(long long own, long long red) {
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int q = threadIdx.x + n * THREADS, row = q / kRowPieces, c = q % kRowPieces;
+            const long long row_left = (TR ? red : own) - row, left = (TR ? own : red) - c * V;
+            x[n] = u32x4{0, 0, 0, 0};
+            if (row_left > 0 && left > 0) {
+                if (VEC) {
+                    x[n] = *reinterpret_cast<const u32x4 *>(src[n]);
+                } else if (left >= V) {
+                    x[n] = *reinterpret_cast<const u32x4_a2 *>(src[n]);
+                } else {
+                    union { u32x4 raw; T e[V]; } p;
+                    p.raw = x[n];
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (i < left) p.e[i] = src[n][i];
+                    x[n] = p.raw;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void advance(long long ld) {
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) src[n] += TR ? BK * ld : BK;
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int q = threadIdx.x + n * THREADS;
+            *reinterpret_cast<u32x4 *>(lds + place<T, TR, N>(q / kRowPieces, q % kRowPieces)) = x[n];
+        }
+    }
+};
+
+// The lane's piece of an operand for matrix step kk (0, 1) of a staged tile: own index `own0 + lane % 16`, 16-bit: reduction indexes
+// 32 kk + 8 (lane / 16) + 0..7, f32: 16 kk + 4 (lane / 16) + 0..3.
+template <typename T, bool TR, int N>
+__device__ __forceinline__ typename Mat<T>::frag read_frag(const char *lds, int own0, int kk) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    union { u32x4 raw; i16x4 half[2]; float f[4]; typename Mat<T>::frag v; } x;
+    if (!TR) {
+        x.raw = *reinterpret_cast<const u32x4 *>(lds + place<T, false, N>(own0 + i, g + 4 * kk));
+    } else if (sizeof(T) == 2) {
+        const int r = 32 * kk + 8 * g + (i >> 2);
+        const int at = place<T, true, N>(r, (own0 >> 4) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+        constexpr int kRowBytes = N * 2;
+        x.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + at));
+        x.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + at + 4 * kRowBytes));     // rows 4 on: the same swizzle
+    } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int r = 16 * kk + 4 * g + s;
+            x.f[s] = *reinterpret_cast<const float *>(lds + place<T, true, N>(r, (own0 + i) >> 2) + ((own0 + i) & 3) * 4);
+        }
+    }
+    return x.v;
+}
+
+// The workgroup's place in the run of its XCD: workgroups go round robin over 8 XCDs, each gets a contiguous run of `total` tiles.
+__device__ __forceinline__ int xcd_tile(int block, int total) {
+    const int per = total >> 3, rest = total & 7, xcd = block & 7, k = block >> 3;
+    return xcd * per + (xcd < rest ? xcd : rest) + k;
+}
+__device__ __forceinline__ bool xcd_has(int block, int total) { return (block >> 3) < (total >> 3) + ((block & 7) < (total & 7) ? 1 : 0); }
+
+enum { PRODUCT_ROWS = 0, PRODUCT_WEIGHTS = 1 };
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, bool VEC, int PRODUCT>
+__global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(const GroupedArgs a) {
+    constexpr int THREADS = (BI / WI) * (BJ / WJ) * 64, BK = 128 / sizeof(T);
+    constexpr int FI = WI / 16, FJ = WJ / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tiles_i = (a.ni + BI - 1) / BI;
+    const T *base_i = static_cast<const T *>(a.I), *base_j = static_cast<const T *>(a.J);
+    int it, group;
+    long long j0, j_left, r0, red;                         // first output row and how many are left, first reduction index and their number
+    long long out_row;
+    if (PRODUCT == PRODUCT_ROWS) {
+        int total = 0;                                     // row tiles of all groups
+        for (int b = 0; b < a.groups; b += 64) {
+            int n = 0;
+            if (b + lane < a.groups) {
+                const long long rows = offset_at(a, b + lane + 1) - offset_at(a, b + lane);
+                n = rows > 0 ? static_cast<int>((rows + BJ - 1) / BJ) : 0;
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off);
+            total += n;
+        }
+        // rows of no group: before the first, behind the last
+        const long long head = offset_at(a, 0), tail = offset_at(a, a.groups);
+        const long long stray = (head + (a.rows - tail)) * a.ni;
+        for (long long e = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; e < stray; e += static_cast<long long>(gridDim.x) * THREADS) {
+            const long long r = e / a.ni, row = r < head ? r : tail + (r - head);
+            static_cast<T *>(a.out)[row * a.ld_out + e % a.ni] = static_cast<T>(0.0f);
+        }
+        total *= tiles_i;
+        if (!xcd_has(blockIdx.x, total)) return;
+        const int tile = xcd_tile(blockIdx.x, total);
+        int before = 0, mine = 0;
+        group = 0;
+        for (int b = 0; b < a.groups; b += 64) {
+            int n = 0;
+            if (b + lane < a.groups) {
+                const long long rows = offset_at(a, b + lane + 1) - offset_at(a, b + lane);
+                n = rows > 0 ? static_cast<int>((rows + BJ - 1) / BJ) : 0;
+            }
+            int upto = n;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int y = __shfl_up(upto, off);
+                if (lane >= off) upto += y;
+            }
+            const unsigned long long past = __ballot((before + upto) * tiles_i > tile);
+            if (past) {
+                const int l = __ffsll(past) - 1;
+                group = b + l;
+                mine = __shfl(n, l);
+                before += __shfl(upto, l) - mine;
+                break;
+            }
+            before += __shfl(upto, 63);
+        }
+        // the row tiles of a group go fastest: they share the weights' tile
+        const int local = tile - before * tiles_i;
+        it = local / mine;
+        const long long row0 = offset_at(a, group), rows = offset_at(a, group + 1) - row0;
+        j0 = row0 + static_cast<long long>(local % mine) * BJ;
+        j_left = row0 + rows - j0;
+        r0 = 0;
+        red = a.red;
+        out_row = j0;
+        base_i += static_cast<long long>(group) * (TRI ? a.red : a.ni) * a.ld_i;
+    } else {
+        const int tiles_j = (a.nj + BJ - 1) / BJ, per_group = tiles_i * tiles_j;
+        int tile = xcd_tile(blockIdx.x, gridDim.x);
+        const int split = tile % a.splits;
+        tile /= a.splits;
+        group = tile / per_group;
+        const int local = tile % per_group;
+        it = local % tiles_i;
+        j0 = static_cast<long long>(local / tiles_i) * BJ;
+        j_left = a.nj - j0;
+        const long long row0 = offset_at(a, group);
+        long long rows = offset_at(a, group + 1) - row0;
+        if (rows < 0) rows = 0;
+        const long long len = ((rows + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+        r0 = row0 + split * len;
+        red = rows - split * len < len ? rows - split * len : len;
+        out_row = (static_cast<long long>(split) * a.groups + group) * a.nj + j0;
+    }
+    const long long i0 = static_cast<long long>(it) * BI, i_left = a.ni - i0;
+
+    f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int fi = 0; fi < FI; ++fi)
+#pragma unroll
+        for (int fj = 0; fj < FJ; ++fj) acc[fi][fj] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int wi = (wave % (BI / WI)) * WI, wj = (wave / (BI / WI)) * WJ;
+    constexpr int kBuffer = (BI + BJ) * 128, kJ = BI * 128;                 // two buffers, I's tile in front of J's
+    const int steps = red > 0 ? static_cast<int>((red + BK - 1) / BK) : 0;
+    if (steps > 0) {
+        Stage<T, TRI, BI, THREADS, VEC> si;
+        Stage<T, TRJ, BJ, THREADS, VEC> sj;
+        si.init(base_i, a.ld_i, i0, r0);
+        sj.init(base_j, a.ld_j, j0, r0);
+        si.load(i_left, red);
+        sj.load(j_left, red);
+        si.store(lds);
+        sj.store(lds + kJ);
+        __syncthreads();
+        for (int t = 0; t < steps; ++t) {
+            const bool more = t + 1 < steps;
+            if (more) {
+                si.advance(a.ld_i);
+                sj.advance(a.ld_j);
+                const long long left = red - static_cast<long long>(t + 1) * BK;
+                si.load(i_left, left);
+                sj.load(j_left, left);
+            }
+            const char *li = lds + (t & 1) * kBuffer, *lj = li + kJ;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                typename Mat<T>::frag fi[FI], fj[FJ];
+#pragma unroll
+                for (int x = 0; x < FI; ++x) fi[x] = read_frag<T, TRI, BI>(li, wi + 16 * x, kk);
+#pragma unroll
+                for (int x = 0; x < FJ; ++x) fj[x] = read_frag<T, TRJ, BJ>(lj, wj + 16 * x, kk);
+#pragma unroll
+                for (int x = 0; x < FI; ++x)
+#pragma unroll
+                    for (int y = 0; y < FJ; ++y) Mat<T>::mma(acc[x][y], fi[x], fj[y]);
+            }
+            if (more) {
+                char *next = lds + ((t + 1) & 1) * kBuffer;
+                si.store(next);
+                sj.store(next + kJ);
+            }
+            __syncthreads();
+        }
+    }
+    // a lane has elements i .. i + 3 of output row j
+#pragma unroll
+    for (int fi = 0; fi < FI; ++fi) {
+        const int i = wi + 16 * fi + 4 * (lane >> 4);
+        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (PRODUCT == PRODUCT_ROWS && a.bias) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < i_left) b[k] = static_cast<float>(static_cast<const T *>(a.bias)[static_cast<long long>(group) * a.ni + i0 + i + k]);
+        }
+#pragma unroll
+        for (int fj = 0; fj < FJ; ++fj) {
+            const int j = wj + 16 * fj + (lane & 15);
+            if (j >= j_left || i >= i_left) continue;
+            const long long at = (out_row + j) * a.ld_out + i0 + i;
+            if (PRODUCT == PRODUCT_WEIGHTS && a.splits > 1) {
+                float *dst = static_cast<float *>(a.out) + at;
+                typedef float four_t __attribute__((ext_vector_type(4), aligned(4)));
+                if (i + 4 <= i_left) *reinterpret_cast<four_t *>(dst) = acc[fi][fj];
+                else
+                    for (int k = 0; k < 4; ++k)
+                        if (i + k < i_left) dst[k] = acc[fi][fj][k];
+            } else {
+                T *dst = static_cast<T *>(a.out) + at;
+                typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+                four_t v;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = static_cast<T>(acc[fi][fj][k] + b[k]);
+                if (i + 4 <= i_left) *reinterpret_cast<four_t *>(dst) = v;
+                else
+                    for (int k = 0; k < 4; ++k)
+                        if (i + k < i_left) dst[k] = v[k];
+            }
+        }
+    }
+}
+
+// out[e] = sum over the splits, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void oc_grouped_join_kernel(const float *parts, T *out, long long n, int splits) {
+    for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < n; e += static_cast<long long>(gridDim.x) * 256) {
+        float s = 0.0f;
+        for (int k = 0; k < splits; ++k) s += parts[k * n + e];
+        out[e] = static_cast<T>(s);
+    }
+}
+
+// Column sums of dY per group: a block has 64 columns of one group and one split of its rows; 4 columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void oc_grouped_bias_kernel(const GroupedArgs a) {
+    __shared__ float part[16][64];
+    const int blocks_i = (a.ni + 63) / 64;
+    const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, group = tile / blocks_i;
+    const int c0 = (tile % blocks_i) * 64 + (threadIdx.x & 15) * 4, lane_row = threadIdx.x >> 4;
+    const long long row0 = offset_at(a, group);
+    long long rows = offset_at(a, group + 1) - row0;
+    if (rows < 0) rows = 0;
+    const long long len = (rows + a.splits - 1) / a.splits, first = split * len, last = first + len < rows ? first + len : rows;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const T *src = static_cast<const T *>(a.J);
+    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (c0 + 4 <= a.ni) {
+#pragma unroll 4
+        for (long long r = first + lane_row; r < last; r += 16) {
+            const four_t v = *reinterpret_cast<const four_t *>(src + (row0 + r) * a.ld_j + c0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += static_cast<float>(v[k]);
+        }
+    } else {
+        for (long long r = first + lane_row; r < last; r += 16)
+            for (int k = 0; k < 4; ++k)
+                if (c0 + k < a.ni) s[k] += static_cast<float>(src[(row0 + r) * a.ld_j + c0 + k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[lane_row][(threadIdx.x & 15) * 4 + k] = s[k];
+    __syncthreads();
+    const int c = (tile % blocks_i) * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && c < a.ni) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += part[k][threadIdx.x];
+        if (a.splits > 1) static_cast<float *>(a.out)[(static_cast<long long>(split) * a.groups + group) * a.ni + c] = sum;
+        else static_cast<T *>(a.out)[static_cast<long long>(group) * a.ni + c] = static_cast<T>(sum);
+    }
+}
+
+template <typename K>
+hipError_t launch_tiles(K kernel, int threads, int lds_bytes, long long blocks, const GroupedArgs &a, hipStream_t s) {
+    if (blocks <= 0) return hipSuccess;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (lds_bytes > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes);
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<dim3(static_cast<unsigned>(blocks)), threads, lds_bytes, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PRODUCT>
+hipError_t launch_product(const GroupedArgs &a, bool vec, hipStream_t s) {
+    constexpr int threads = (BI / WI) * (BJ / WJ) * 64, lds = 2 * (BI + BJ) * 128;
+    const long long tiles_i = (a.ni + BI - 1) / BI;
+    const long long blocks = PRODUCT == PRODUCT_ROWS ? (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i
+                                                     : tiles_i * ((a.nj + BJ - 1) / BJ) * a.groups * a.splits;
+    return vec ? launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, true, PRODUCT>, threads, lds, blocks, a, s)
+               : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, false, PRODUCT>, threads, lds, blocks, a, s);
+}
+
+// Which tile: few rows a group -- narrow in rows, many workgroups, the weights stream through; enough work to fill the 256 CUs with
+// 256 x 256 tiles (16-bit types) -- those; else 128 x 128.
+template <typename T, bool TRI, bool TRJ>
+hipError_t launch_rows(const GroupedArgs &a, bool vec, hipStream_t s) {
+    if (a.rows <= 32LL * a.groups) return launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+    if constexpr (sizeof(T) == 2) {
+        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+    }
+    if (a.ni <= 64) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+    return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+}
+
+struct WeightPlan { int tile, splits, bias_splits; };
+
+// The tile of dW and into how many pieces its rows are cut so that there are workgroups for every CU (a piece has 128 rows or more).
+WeightPlan weight_plan(int type, long long rows, int groups, int ni, int nj) {
+    WeightPlan p;
+    const auto tiles = [&](int b) { return static_cast<long long>((ni + b - 1) / b) * ((nj + b - 1) / b) * groups; };
+    p.tile = type != OC_F32 && ni > 128 && nj > 128 && tiles(256) >= 224 ? 256 : ni <= 64 || nj <= 64 ? 64 : 128;
+    const long long most = std::max<long long>(1, rows / groups / 128);
+    const auto cut = [&](long long blocks) { return static_cast<int>(std::max<long long>(1, std::min<long long>({most, (512 + blocks - 1) / blocks, 64}))); };
+    p.splits = tiles(p.tile) >= 224 ? 1 : cut(tiles(p.tile));
+    const long long bias_blocks = static_cast<long long>((nj + 63) / 64) * groups;
+    p.bias_splits = bias_blocks >= 512 ? 1 : cut(bias_blocks);
+    return p;
+}
+
+template <typename T>
+hipError_t launch_weights(const GroupedArgs &a, const WeightPlan &p, bool vec, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS>(a, vec, s);
+    }
+    if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS>(a, vec, s);
+    return launch_product<T, 128, 128, 64, 64, true, true, PRODUCT_WEIGHTS>(a, vec, s);
+}
+
+template <typename T>
+hipError_t launch_join(const float *parts, void *out, long long n, int splits, hipStream_t s) {
+    const int blocks = static_cast<int>(std::min<long long>(4096, (n + 255) / 256));
+    oc_grouped_join_kernel<T><<<dim3(blocks), 256, 0, s>>>(parts, static_cast<T *>(out), n, splits);
+    return hipGetLastError();
+}
+
+bool aligned_rows(const void *p, long long ld, int type) {
+    const long long size = type == OC_F32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+}
+
+int check_grouped(const oc_grouped_linear_args *p, const char *who) {
+    if (!p) return oc_internal_fail(OC_ERR_INVALID_ARG, "%s: NULL arguments", who);
+    if (p->rows < 0 || p->groups < 1 || p->in_features < 1 || p->out_features < 1 || p->type < OC_F32 || p->type > OC_F16 || p->x_stride < p->in_features)
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "%s: rows %lld, groups %d, in_features %d, out_features %d, type %d, x_stride %lld", who,
+                                static_cast<long long>(p->rows), p->groups, p->in_features, p->out_features, p->type, static_cast<long long>(p->x_stride));
+    if (!p->d_weight || !p->d_offsets || (p->rows > 0 && !p->d_x))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "%s: a required pointer is NULL", who);
+    return OC_OK;
+}
+
+template <typename T>
+hipError_t forward_type(const GroupedArgs &a, bool vec, hipStream_t s) { return launch_rows<T, false, false>(a, vec, s); }
+
+template <typename T>
+hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &base, float *parts, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    const int K = p->in_features, N = p->out_features, V = p->type == OC_F32 ? 4 : 8;
+    if (p->d_dx && p->rows > 0) {
+        GroupedArgs a = base;
+        a.I = p->d_weight; a.J = p->d_dy; a.out = p->d_dx;
+        a.ld_i = K; a.ld_j = N; a.ld_out = K;
+        a.ni = K; a.red = N;
+        e = launch_rows<T, true, false>(a, aligned_rows(p->d_weight, K, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
+        if (e != hipSuccess) return e;
+    }
+    const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
+    if (p->d_dweight) {
+        GroupedArgs a = base;
+        a.I = p->d_x; a.J = p->d_dy;
+        a.ld_i = p->x_stride; a.ld_j = N; a.ld_out = K;
+        a.ni = K; a.nj = N; a.splits = plan.splits;
+        a.out = plan.splits > 1 ? static_cast<void *>(parts) : p->d_dweight;
+        e = launch_weights<T>(a, plan, aligned_rows(p->d_x, p->x_stride, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
+        const long long n = static_cast<long long>(p->groups) * N * K;
+        if (e == hipSuccess && plan.splits > 1) e = launch_join<T>(parts, p->d_dweight, n, plan.splits, s);
+        if (e != hipSuccess) return e;
+        parts += plan.splits > 1 ? plan.splits * n : 0;
+    }
+    if (p->d_dbias) {
+        GroupedArgs a = base;
+        a.J = p->d_dy; a.ld_j = N; a.ni = N; a.splits = plan.bias_splits;
+        a.out = plan.bias_splits > 1 ? static_cast<void *>(parts) : p->d_dbias;
+        oc_grouped_bias_kernel<T><<<dim3(static_cast<unsigned>((N + 63) / 64 * static_cast<long long>(p->groups) * plan.bias_splits)), 256, 0, s>>>(a);
+        e = hipGetLastError();
+        if (e == hipSuccess && plan.bias_splits > 1) e = launch_join<T>(parts, p->d_dbias, static_cast<long long>(p->groups) * N, plan.bias_splits, s);
+    }
+    return e;
+}
+
+}  // namespace
+
+extern "C" int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *p) {
+    if (check_grouped(p, "oc_grouped_linear_workspace_bytes") != OC_OK) return -1;
+    const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, p->in_features, p->out_features);
+    const long long out = static_cast<long long>(p->groups) * p->out_features;
+    return ((plan.splits > 1 ? plan.splits * out * p->in_features : 0) + (plan.bias_splits > 1 ? plan.bias_splits * out : 0)) * static_cast<long long>(sizeof(float));
+}
+
+extern "C" int oc_grouped_linear(const oc_grouped_linear_args *p, void *stream) {
+    if (const int rc = check_grouped(p, "oc_grouped_linear")) return rc;
+    if (p->rows == 0) return OC_OK;
+    if (!p->d_y) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear: d_y is NULL");
+    GroupedArgs a = {};
+    a.I = p->d_weight; a.J = p->d_x; a.bias = p->d_bias; a.out = p->d_y; a.offsets = p->d_offsets;
+    a.ld_i = p->in_features; a.ld_j = p->x_stride; a.ld_out = p->out_features;
+    a.rows = p->rows; a.groups = p->groups; a.ni = p->out_features; a.red = p->in_features;
+    a.offsets64 = p->offsets64 != 0; a.splits = 1;
+    const int V = p->type == OC_F32 ? 4 : 8;
+    const bool vec = aligned_rows(p->d_weight, p->in_features, p->type) && aligned_rows(p->d_x, p->x_stride, p->type) && p->in_features % V == 0;
+    const OcDeviceScope on_device(oc_device_of_pointer(p->d_y));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const hipError_t e = p->type == OC_F32 ? forward_type<float>(a, vec, s) : p->type == OC_BF16 ? forward_type<__bf16>(a, vec, s) : forward_type<_Float16>(a, vec, s);
+    return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grouped_linear: %s", hipGetErrorString(e));
+}
+
+extern "C" int oc_grouped_linear_backward(const oc_grouped_linear_args *p, void *d_workspace, void *stream) {
+    if (const int rc = check_grouped(p, "oc_grouped_linear_backward")) return rc;
+    if (p->rows > 0 && !p->d_dy) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: d_dy is NULL");
+    const int64_t need = oc_grouped_linear_workspace_bytes(p);
+    if (need > 0 && (p->d_dweight || p->d_dbias) && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: needs a workspace of %lld bytes", static_cast<long long>(need));
+    GroupedArgs a = {};
+    a.offsets = p->d_offsets; a.rows = p->rows; a.groups = p->groups; a.offsets64 = p->offsets64 != 0; a.splits = 1;
+    const OcDeviceScope on_device(oc_device_of_pointer(p->d_weight));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    float *parts = static_cast<float *>(d_workspace);
+    const hipError_t e = p->type == OC_F32 ? backward_type<float>(p, a, parts, s) : p->type == OC_BF16 ? backward_type<__bf16>(p, a, parts, s)
+                                                                                                       : backward_type<_Float16>(p, a, parts, s);
+    return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grouped_linear_backward: %s", hipGetErrorString(e));
+}

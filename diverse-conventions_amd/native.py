@@ -24,7 +24,7 @@ DIAGNOSTICS = os.environ.get("OC_DIAGNOSTICS", "0") not in ("", "0")
 LIB_OVERRIDE = os.environ.get("OC_LIB_PATH", "")
 LIB_PATH = LIB_OVERRIDE or os.path.join(CSRC, "liboc_hip_asan.so" if SANITIZE else "liboc_hip_diag.so" if DIAGNOSTICS else "liboc_hip.so")
 SOURCES = [os.path.join(CSRC, "overcooked_engine.hip"), os.path.join(CSRC, "rollout_ops.hip"),
-           os.path.join(CSRC, "policy_ops.hip"), os.path.join(CSRC, "update_ops.hip")]
+           os.path.join(CSRC, "policy_ops.hip"), os.path.join(CSRC, "update_ops.hip"), os.path.join(CSRC, "grouped_ops.hip")]
 HEADERS = [os.path.join(CSRC, "policy_pack.h"), os.path.join(CSRC, "oc_internal.h"), os.path.join(CSRC, "policy_block_body.h"), os.path.join(CSRC, "policy_mono_loop.h"),
            os.path.join(CSRC, "policy_duo_kernel.h"), os.path.join(CSRC, "policy_duo_body.h"),
            os.path.join(CSRC, "oc_np_kernels.h")]
@@ -57,6 +57,7 @@ SYMBOLS_ENV = [
 SYMBOLS_OPS = [
     "oc_gae_returns", "oc_advantage_workspace_bytes", "oc_advantage_normalize", "oc_gather_rows", "oc_gather_columns", "oc_pack_columns", "oc_gather_records",
     "oc_policy_loss_workspace_bytes", "oc_policy_loss", "oc_value_loss_workspace_bytes", "oc_value_loss", "oc_grad_norm_workspace_bytes", "oc_grad_norm_clip",
+    "oc_grouped_linear_workspace_bytes", "oc_grouped_linear", "oc_grouped_linear_backward",
     "oc_policy_packed_bytes", "oc_policy_pack_host", "oc_policy_pack", "oc_policy_plan_tiles", "oc_policy_forward", "oc_policy_forward_multi",
     "oc_policy_plan_tiles_multi", "oc_group_policy_rollout_multi", "oc_policy_uniform", "oc_policy_rollout", "oc_group_policy_rollout",
     "oc_partition_rows", "oc_policy_forward_gather", "oc_policy_rollout_mixed",
@@ -107,6 +108,14 @@ class OcValueLossArgs(ctypes.Structure):
                 ("d_loss", ctypes.c_void_p), ("d_weight", ctypes.c_void_p), ("d_grad", ctypes.c_void_p), ("d_grad_out", ctypes.c_void_p), ("n", ctypes.c_int64),
                 ("values_type", ctypes.c_int32), ("clip_param", ctypes.c_float), ("huber_delta", ctypes.c_float), ("mean", ctypes.c_float),
                 ("std", ctypes.c_float), ("grad_scale", ctypes.c_float)]
+
+
+class OcGroupedLinearArgs(ctypes.Structure):
+    """oc_grouped_linear_args"""
+    _fields_ = [("d_x", ctypes.c_void_p), ("d_weight", ctypes.c_void_p), ("d_bias", ctypes.c_void_p), ("d_offsets", ctypes.c_void_p),
+                ("d_y", ctypes.c_void_p), ("d_dy", ctypes.c_void_p), ("d_dx", ctypes.c_void_p), ("d_dweight", ctypes.c_void_p),
+                ("d_dbias", ctypes.c_void_p), ("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("groups", ctypes.c_int32),
+                ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32), ("type", ctypes.c_int32), ("offsets64", ctypes.c_int32)]
 
 
 class OcLayoutParams(ctypes.Structure):
@@ -248,6 +257,11 @@ def lib():
     L.oc_grad_norm_workspace_bytes.argtypes = [ctypes.c_int32]
     L.oc_grad_norm_workspace_bytes.restype = i64
     L.oc_grad_norm_clip.argtypes = [ctypes.c_int32, vp, vp, vp, vp, fp, i32, vp, vp, vp]
+    pg = ctypes.POINTER(OcGroupedLinearArgs)
+    L.oc_grouped_linear_workspace_bytes.argtypes = [pg]
+    L.oc_grouped_linear_workspace_bytes.restype = i64
+    L.oc_grouped_linear.argtypes = [pg, vp]
+    L.oc_grouped_linear_backward.argtypes = [pg, vp, vp]
     ps = ctypes.POINTER(OcPolicyShape)
     L.oc_policy_packed_bytes.argtypes = [ps]
     L.oc_policy_packed_bytes.restype = i64

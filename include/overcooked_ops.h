@@ -134,6 +134,29 @@ int64_t oc_grad_norm_workspace_bytes(int32_t n_tensors);
 int oc_grad_norm_clip(int32_t n_tensors, const void *const *d_grads, void *const *d_out, const int64_t *numel, const int32_t *types,
                       float max_norm, int inf_norm, float *d_norm, void *d_workspace, void *stream);
 
+/* Linear layers of several networks over one batch whose rows are sorted by network, with their gradients: training's counterpart of the
+ * (row range, network) tables of oc_policy_forward -- the critics of all pairing segments learn at once instead of one after the other
+ * (train/XD/xd.py updates sp_critic, xp_critic0[i], xp_critic1[i] in turn).
+ *   forward:   y[r] = x[r] weight[g]^T + bias[g]          for d_offsets[g] <= r < d_offsets[g + 1]; rows of no group are 0
+ *   backward:  dx[r] = dy[r] weight[g];  dweight[g] = sum_r dy[r]^T x[r];  dbias[g] = sum_r dy[r]  (each left out where its pointer is NULL)
+ * Products run on the matrix cores with f32 accumulation; results are rounded once.  d_offsets [groups + 1] must not decrease; entries
+ * are clamped into [0, rows], a group may be empty (its gradients are 0).  dweight and dbias of few, long groups are summed in f32
+ * pieces through the workspace (oc_grouped_linear_workspace_bytes, 0 if none is needed), in a fixed order. */
+typedef struct {
+    const void *d_x;                   /* [rows] of in_features values, x_stride elements apart */
+    const void *d_weight;              /* [groups][out_features][in_features] */
+    const void *d_bias;                /* [groups][out_features] or NULL */
+    const void *d_offsets;             /* [groups + 1] int32, or int64 with offsets64 */
+    void *d_y;                         /* [rows][out_features] */
+    const void *d_dy;                  /* [rows][out_features] */
+    void *d_dx, *d_dweight, *d_dbias;  /* as x (contiguous), weight, bias; or NULL */
+    int64_t rows, x_stride;
+    int32_t groups, in_features, out_features, type, offsets64;
+} oc_grouped_linear_args;
+int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *args);
+int oc_grouped_linear(const oc_grouped_linear_args *args, void *stream);
+int oc_grouped_linear_backward(const oc_grouped_linear_args *args, void *d_workspace, void *stream);
+
 /* ---- fused policy inference on the matrix cores --------------------------------------------
  * One launch evaluates every (row range, network) tile of a rollout step -- all conventions' actors and critics,
  * both sides, every pairing segment -- reading the int8 observations oc_step wrote and writing the int32 actions
