@@ -32,13 +32,29 @@ template <typename T> struct Chunk {                       // 16 bytes of elemen
     __device__ Chunk() {}
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e30f;                          // floor of log-probabilities in products with a probability of 0
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+// The hardware's own exp2, log2 and reciprocal: 1 ulp, where arguments below the normal range do not matter (a probability of 2^-127
+// counts as 0 next to one of 1).  The library functions around them cost more than the memory traffic of a short row.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e); }
+__device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// A row's logits as exponents of 2 relative to its largest, v = z scale + shift in one fma.  Scale is log2 e; a largest logit beyond
+// 1e38 (a row at the type's lowest value, say) would leave the range with it, but there two logits are equal or 1e31 apart, and any scale
+// keeps exp2(v) at 1 or 0.
+struct Exponent { float scale, shift; };
+__device__ __forceinline__ Exponent exponent_of(float m) {
+    Exponent x;
+    x.scale = fabsf(m) < 1e38f || m == __builtin_inff() ? kLog2e : 0x1p-20f;
+    x.shift = m == neg_inf() ? 0.0f : -m * x.scale;
+    return x;
+}
 
 constexpr int kMaxBlocks = 2048;                           // of a launch that leaves one set of partial sums per block
-constexpr int kWeightBlocks = 256;                         // of the launch that adds up the weights
+constexpr int kWeightBlocks = 1024;                        // of the launch that adds up the weights
 constexpr int kSums = 6;
 
 struct PolicyLossArgs {
@@ -80,18 +96,36 @@ __device__ __forceinline__ double block_sum(double x, double *part) {
     return x;
 }
 
+// The same for N values with one exchange, valid in threads 0 .. N - 1: thread i returns value i.
+template <int N>
+__device__ __forceinline__ double block_sums(const double (&x)[N], double (*part)[N]) {
+    double y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = x[i];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] += __shfl_xor(y[i], off);
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[threadIdx.x >> 6][i] = y[i];
+    __syncthreads();
+    double sum = 0.0;
+    if (threadIdx.x < N)
+        for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) sum += part[w][threadIdx.x];
+    return sum;
+}
+
 // The taken action of a row, -1 when it is none of 0 .. n - 1 (also a float that is NaN or lies outside).
-__device__ __forceinline__ int action_of(const PolicyLossArgs &a, long long row) {
-    long long v;
-    if (a.action_type == OC_ACT_F32) {
-        const float f = static_cast<const float *>(a.actions)[row];
-        v = f > -1.0f && f < static_cast<float>(a.n_actions) ? static_cast<long long>(f) : -1;
-    } else if (a.action_type == OC_ACT_I64) {
-        v = static_cast<const long long *>(a.actions)[row];
-    } else {
-        v = static_cast<const int *>(a.actions)[row];
-    }
-    return v >= 0 && v < a.n_actions ? static_cast<int>(v) : -1;
+__device__ __forceinline__ int checked_action(int v, int n) { return v >= 0 && v < n ? v : -1; }
+__device__ __forceinline__ int checked_action(long long v, int n) { return v >= 0 && v < n ? static_cast<int>(v) : -1; }
+__device__ __forceinline__ int checked_action(float f, int n) { return f > -1.0f && f < static_cast<float>(n) ? static_cast<int>(f) : -1; }
+
+// `first`: a row that is the same for all lanes, `i`: this lane's behind it
+__device__ __forceinline__ int action_of(const PolicyLossArgs &a, long long first, uint32_t i = 0) {
+    if (a.action_type == OC_ACT_F32) return checked_action((static_cast<const float *>(a.actions) + first)[i], a.n_actions);
+    if (a.action_type == OC_ACT_I64) return checked_action((static_cast<const long long *>(a.actions) + first)[i], a.n_actions);
+    return checked_action((static_cast<const int *>(a.actions) + first)[i], a.n_actions);
 }
 
 __device__ __forceinline__ double row_weight(const PolicyLossArgs &a, long long row) {
@@ -99,11 +133,37 @@ __device__ __forceinline__ double row_weight(const PolicyLossArgs &a, long long 
     return a.weights ? static_cast<double>(a.weights[row]) : 1.0;
 }
 
+// Weights of four rows, in 16-byte loads.
+__device__ __forceinline__ double four_weights(const PolicyLossArgs &a, long long row) {
+    const u32x4 w = a.weights ? *reinterpret_cast<const u32x4_a4 *>(a.weights + row) : u32x4{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u};
+    int v[4];
+    if (a.action_type == OC_ACT_I64) {
+        const u32x4 x = reinterpret_cast<const u32x4_a4 *>(static_cast<const long long *>(a.actions) + row)[0];
+        const u32x4 y = reinterpret_cast<const u32x4_a4 *>(static_cast<const long long *>(a.actions) + row)[1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[i] = checked_action(static_cast<long long>(static_cast<uint64_t>(x[2 * i + 1]) << 32 | x[2 * i]), a.n_actions);
+            v[2 + i] = checked_action(static_cast<long long>(static_cast<uint64_t>(y[2 * i + 1]) << 32 | y[2 * i]), a.n_actions);
+        }
+    } else {
+        const u32x4 x = *reinterpret_cast<const u32x4_a4 *>(static_cast<const int *>(a.actions) + row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a.action_type == OC_ACT_F32 ? checked_action(__uint_as_float(x[i]), a.n_actions) : checked_action(static_cast<int>(x[i]), a.n_actions);
+    }
+    double sum[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i & 1] += v[i] >= 0 ? static_cast<double>(__uint_as_float(w[i])) : 0.0;
+    return sum[0] + sum[1];
+}
+
 __global__ __launch_bounds__(256) void oc_policy_weight_kernel(const PolicyLossArgs a) {
     __shared__ double part[4];
     double w = 0.0;
     const long long stride = static_cast<long long>(gridDim.x) * 256;
-    for (long long r = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; r < a.rows; r += stride) w += row_weight(a, r);
+    const long long quads = a.rows >> 2;
+#pragma unroll 4
+    for (long long q = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; q < quads; q += stride) w += four_weights(a, q << 2);
+    if (blockIdx.x == 0 && threadIdx.x < (a.rows & 3)) w += row_weight(a, (quads << 2) + threadIdx.x);
     w = block_sum(w, part);
     if (threadIdx.x == 0) a.weight_partials[blockIdx.x] = w;
 }
@@ -123,64 +183,70 @@ __device__ __forceinline__ float inverse_weight(const PolicyLossArgs &a, double 
     return w != 0.0 ? static_cast<float>(1.0 / w) : 0.0f;
 }
 
-// What the rows of a thread (or of a group's first lane) add to the sums.
+// What the rows of a thread (or of a group's first lane) add to the sums; a group's lane keeps them in LDS.
 struct RowSums {
-    double policy = 0, entropy = 0, kl = 0, clipped = 0, ratio = 0, weight = 0;
+    double s[kSums];                                       // policy, entropy, kl, clipped, ratio, weight
 };
 
-__device__ __forceinline__ void write_result(const PolicyLossArgs &a, const double (&s)[kSums]) {
-    const double inv = s[5] != 0.0 ? 1.0 / s[5] : 0.0;
-    double loss = s[0];                                    // a term without weight stays out, also where it is not finite
-    if (a.entropy_coef != 0.0f) loss -= static_cast<double>(a.entropy_coef) * s[1];
-    if (a.kl_coef != 0.0f) loss += static_cast<double>(a.kl_coef) * s[2];
-    *a.loss = static_cast<float>(loss * inv);
-    if (a.stats)
-#pragma unroll
-        for (int i = 0; i < 5; ++i) a.stats[i] = static_cast<float>(s[i] * inv);
-    if (a.weight) *a.weight = s[5];
-}
-
-__device__ __forceinline__ void finish_sums(const PolicyLossArgs &a, const RowSums &r, double *part) {
-    if (!a.want_sums) return;
-    double s[kSums] = {r.policy, r.entropy, r.kl, r.clipped, r.ratio, r.weight};
-#pragma unroll
-    for (int i = 0; i < kSums; ++i) s[i] = block_sum(s[i], part);
-    if (threadIdx.x != 0) return;
-    if (a.finalize_here) {
-        write_result(a, s);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kSums; ++i) a.sums[static_cast<long long>(blockIdx.x) * kSums + i] = s[i];
+// The results from the six sums: thread i has sum i.
+__device__ __forceinline__ void write_result(const PolicyLossArgs &a, double mine) {
+    if (threadIdx.x >= 64) return;
+    const double weight = __shfl(mine, 5), inv = weight != 0.0 ? 1.0 / weight : 0.0;
+    const double entropy = __shfl(mine, 1), kl = __shfl(mine, 2);
+    if (threadIdx.x == 0) {
+        double loss = mine;                                // a term without weight stays out, also where it is not finite
+        if (a.entropy_coef != 0.0f) loss -= static_cast<double>(a.entropy_coef) * entropy;
+        if (a.kl_coef != 0.0f) loss += static_cast<double>(a.kl_coef) * kl;
+        *a.loss = static_cast<float>(loss * inv);
+        if (a.weight) *a.weight = weight;
     }
+    if (a.stats && threadIdx.x < 5) a.stats[threadIdx.x] = static_cast<float>(mine * inv);
 }
 
-__global__ __launch_bounds__(256) void oc_policy_finalize_kernel(const PolicyLossArgs a, int blocks) {
-    __shared__ double part[4];
+__device__ __forceinline__ void finish_sums(const PolicyLossArgs &a, const RowSums &r, double (*part)[kSums]) {
+    if (!a.want_sums) return;
+    const double mine = block_sums(r.s, part);
+    if (a.finalize_here) write_result(a, mine);
+    else if (threadIdx.x < kSums) a.sums[static_cast<long long>(blockIdx.x) * kSums + threadIdx.x] = mine;
+}
+
+__global__ __launch_bounds__(1024) void oc_policy_finalize_kernel(const PolicyLossArgs a, int blocks) {
+    __shared__ double part[16][kSums];
     double s[kSums] = {0, 0, 0, 0, 0, 0};
-    for (int b = threadIdx.x; b < blocks; b += 256)
+    for (int b = threadIdx.x; b < blocks; b += 1024)
 #pragma unroll
         for (int i = 0; i < kSums; ++i) s[i] += a.sums[static_cast<long long>(b) * kSums + i];
-#pragma unroll
-    for (int i = 0; i < kSums; ++i) s[i] = block_sum(s[i], part);
-    if (threadIdx.x == 0) write_result(a, s);
+    write_result(a, block_sums(s, part));
 }
 
-// One row behind its softmax: `za` the taken action's logit (-inf: not possible), m the largest logit, s = sum exp(z - m),
-// t = sum exp(z - m) (z - m).  Adds to the sums; the gradient of logit j is then p_j (ce (z_j - m) + k) + [j == taken] c1 with
-// p_j = exp(z_j - m) / s:
-//   d loss / d lp = c1 = (w / W) (-A ratio [not clipped] + ck (1 - exp(ref - lp)));  d H / d z_j = -p_j (log p_j + H).
-struct RowGrad { float c1, ce, k, inv_s; };
+// One row behind its softmax, in units of log 2: `va` the exponent of the taken action, s = sum 2^v, t = sum 2^v v over the possible
+// actions.  Adds to the sums; the gradient of logit j is then, times `go`, 2^v_j (a1 v_j + a0) + [j == taken] c1:
+//   d loss / d lp = c1 = (w / W) (-A ratio [not clipped] + ck (1 - exp(ref - lp)));  d H / d z_j = -p_j (log p_j + H),  p_j = 2^v_j / s.
+struct RowGrad {
+    float c1, a1, a0;
+    bool none;                                             // the row adds nothing
+};
 
-__device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, long long row, float weight, float inv_w, float za, float m, float s, float t,
-                                             bool leader, RowSums &sums) {
-    RowGrad g = {0.0f, 0.0f, 0.0f, 0.0f};
-    // nothing is possible, or the taken action is not: the row adds nothing (logits that are all NaN leave m at -inf and s NaN)
-    if ((m == neg_inf() && s == 0.0f) || za == neg_inf()) return g;
-    const float log_s = logf(s);
-    const float lp = (za - m) - log_s;
-    const float entropy = log_s - t / s;
-    const float adv = a.adv[row];
-    const float ratio = expf(lp - a.old_logp[row]);
+struct RowInputs { float weight, adv, old_logp, ref_logp; };
+
+__device__ __forceinline__ RowInputs row_inputs(const PolicyLossArgs &a, long long first, uint32_t i, int action) {
+    RowInputs r;
+    r.weight = action < 0 ? 0.0f : a.weights ? (a.weights + first)[i] : 1.0f;
+    r.adv = (a.adv + first)[i];
+    r.old_logp = (a.old_logp + first)[i];
+    r.ref_logp = a.ref_logp ? (a.ref_logp + first)[i] : 0.0f;
+    return r;
+}
+
+__device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, const RowInputs &in, float inv_w, float go, bool possible, float va, float s,
+                                             float t, bool leader, RowSums &sums) {
+    RowGrad g = {0.0f, 0.0f, 0.0f, true};
+    if (!possible) return g;
+    const float log_s = log2_fast(s), inv_s = rcp_fast(s);
+    const float lp = (va - log_s) * kLn2;
+    const float entropy = (log_s - t * inv_s) * kLn2;
+    const float adv = in.adv, weight = in.weight;
+    const float ratio = exp_fast(lp - in.old_logp);
     const float kept = fminf(fmaxf(ratio, a.clip_lo), a.clip_hi);
     const float s1 = ratio * adv, s2 = kept * adv;
     const float policy = -(s1 != s1 || s2 != s2 ? s1 + s2 : fminf(s1, s2));
@@ -188,25 +254,29 @@ __device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, long long 
     float slope = cut ? 0.0f : -s1;
     float kl = 0.0f;
     if (a.ref_logp) {
-        const float d = a.ref_logp[row] - lp, e = expm1f(d);
+        const float d = in.ref_logp - lp, e = exp_fast(d) - 1.0f;
         kl = e - d;
         if (a.kl_coef != 0.0f) slope = slope - a.kl_coef * e;
     }
     if (leader) {
         const double w = weight;
-        sums.policy += w * policy;
-        sums.entropy += w * entropy;
-        sums.kl += w * kl;
-        sums.clipped += ratio < a.clip_lo || ratio > a.clip_hi ? w : 0.0;
-        sums.ratio += w * ratio;
+        sums.s[0] = fma(w, static_cast<double>(policy), sums.s[0]);
+        sums.s[1] = fma(w, static_cast<double>(entropy), sums.s[1]);
+        sums.s[2] = fma(w, static_cast<double>(kl), sums.s[2]);
+        sums.s[3] += ratio < a.clip_lo || ratio > a.clip_hi ? w : 0.0;
+        sums.s[4] = fma(w, static_cast<double>(ratio), sums.s[4]);
     }
-    const float scale = weight * inv_w;
+    const float scale = weight * inv_w * go;
+    const float ce = scale * a.entropy_coef;
     g.c1 = scale * slope;
-    g.ce = scale * a.entropy_coef;
-    g.k = g.ce * (entropy - log_s) - g.c1;
-    g.inv_s = 1.0f / s;
+    g.a1 = ce * kLn2 * inv_s;
+    g.a0 = (ce * (entropy - log_s * kLn2) - g.c1) * inv_s;
+    g.none = false;
     return g;
 }
+
+// Gradient of a logit with exponent v and e = 2^v; the taken action's c1 comes on top.
+__device__ __forceinline__ float grad_of(const RowGrad &g, float v, float e) { return e * fmaf(g.a1, fmaxf(v, kLowest), g.a0); }
 
 // -------------------------------------------------------------------------------------------------------------------------------
 // Up to 16 actions: a thread has a whole row.  The block's 256 rows are one contiguous piece of memory; it is copied through LDS in
@@ -233,27 +303,43 @@ __device__ __forceinline__ void copy_out(void *dst, const void *lds, int bytes) 
     if (static_cast<int>(threadIdx.x) < bytes - whole) static_cast<char *>(dst)[whole + threadIdx.x] = static_cast<const char *>(lds)[whole + threadIdx.x];
 }
 
-template <typename T, int AM, bool GRAD>
+// EXACT: a row has AM values; else at most AM.
+template <typename T, int AM, bool EXACT, bool GRAD>
 __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLossArgs a) {
     __shared__ __attribute__((aligned(16))) T rows_lds[kRowTile * AM];
     __shared__ __attribute__((aligned(16))) char avail_lds[kRowTile * AM * 4];
-    __shared__ double part[4];
-    const int A = a.n_actions;
+    __shared__ double part[4], parts[4][kSums];
+    const int A = EXACT ? AM : a.n_actions;
     const float inv_w = GRAD ? inverse_weight(a, part) : 0.0f;
     const float go = GRAD ? a.grad_scale * (a.grad_out ? *a.grad_out : 1.0f) : 0.0f;
     const bool stage_avail = a.avail && a.avail_stride == A;
-    RowSums sums;
+    const auto may_at = [&](long long at) {
+        return a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[at] != 0 : static_cast<const float *>(a.avail)[at] != 0.0f;
+    };
+    const uint32_t everything = (1u << A) - 1;
+    uint32_t may_all = everything;                         // a bit per action; one mask for all rows is read once
+    if (a.avail && a.avail_stride == 0) {
+        may_all = 0;
+        for (int j = 0; j < A; ++j) may_all |= may_at(j) ? 1u << j : 0;
+    }
+    RowSums sums = {};
     const long long tiles = (a.rows + kRowTile - 1) / kRowTile;
     for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const long long row0 = tile * kRowTile;
         const int n = static_cast<int>(a.rows - row0 < kRowTile ? a.rows - row0 : kRowTile);
-        const int me = threadIdx.x;
+        int me = threadIdx.x;
+        asm volatile("" : "+v"(me));                       // places are computed anew, not kept in registers over the loop
         const long long row = row0 + me;
         const bool live = me < n;
+        // everything that a row needs is on its way before the first wait
+        const int action = live ? action_of(a, row0, me) : -1;
+        RowInputs in = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (live) in = row_inputs(a, row0, me, action);
         if (a.row_stride == A)
             copy_in<sizeof(T) == 4 ? 4 : 2>(rows_lds, static_cast<const T *>(a.logits) + row0 * A, n * A * static_cast<int>(sizeof(T)));
         else if (live)
             for (int j = 0; j < A; ++j) rows_lds[me * A + j] = static_cast<const T *>(a.logits)[row * a.row_stride + j];
+        uint32_t may = may_all;
         if (stage_avail) {
             const int size = a.avail_u8 ? 1 : 4;
             const char *src = static_cast<const char *>(a.avail) + row0 * A * size;
@@ -262,48 +348,54 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
             } else {
                 copy_in<4>(avail_lds, src, n * A * 4);
             }
+        } else if (a.avail && a.avail_stride != 0 && live) {
+            may = 0;
+            for (int j = 0; j < A; ++j) may |= may_at(row * a.avail_stride + j) ? 1u << j : 0;
         }
-        const int action = live ? action_of(a, row) : -1;
-        const float weight = action < 0 ? 0.0f : a.weights ? a.weights[row] : 1.0f;
         __syncthreads();
         float z[AM];
         float m = neg_inf(), za = neg_inf();
 #pragma unroll
-        for (int j = 0; j < AM; ++j) {
-            z[j] = neg_inf();
-            if (j < A && live) {
-                bool may = true;
-                if (stage_avail)
-                    may = a.avail_u8 ? avail_lds[me * A + j] != 0 : reinterpret_cast<const float *>(avail_lds)[me * A + j] != 0.0f;
-                else if (a.avail)
-                    may = a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[row * a.avail_stride + j] != 0
-                                     : static_cast<const float *>(a.avail)[row * a.avail_stride + j] != 0.0f;
-                if (may) z[j] = static_cast<float>(rows_lds[me * A + j]);
-                if (j == action) za = z[j];
+        for (int j = 0; j < AM; ++j) z[j] = static_cast<float>(rows_lds[me * A + (j < A ? j : 0)]);
+        if (stage_avail) {
+            may = 0;
+            if (a.avail_u8) {
+#pragma unroll
+                for (int j = 0; j < AM; ++j) may |= avail_lds[me * A + (j < A ? j : 0)] != 0 ? 1u << j : 0;
+            } else {
+#pragma unroll
+                for (int j = 0; j < AM; ++j) may |= reinterpret_cast<const float *>(avail_lds)[me * A + (j < A ? j : 0)] != 0.0f ? 1u << j : 0;
             }
+            may &= everything;
+        }
+#pragma unroll
+        for (int j = 0; j < AM; ++j) {
+            z[j] = may >> j & 1 ? z[j] : neg_inf();
+            za = j == action ? z[j] : za;
             m = fmaxf(m, z[j]);
         }
-        RowGrad g = {0.0f, 0.0f, 0.0f, 0.0f};
-        float s = 0.0f, t = 0.0f;
-        if (weight != 0.0f) {
-            sums.weight += weight;
-            const float base = m == neg_inf() ? 0.0f : m;
+        RowGrad g = {0.0f, 0.0f, 0.0f, true};
+        const Exponent x = exponent_of(m);
+        float e[AM], s = 0.0f, t = 0.0f;
+        if (in.weight != 0.0f) {
+            sums.s[5] += in.weight;
 #pragma unroll
             for (int j = 0; j < AM; ++j) {
-                const float u = z[j] - base, e = exp2_fast(u * kLog2e);
-                s += e;
-                t = fmaf(e, fmaxf(u, kLowest), t);
+                const float v = fmaf(z[j], x.scale, x.shift);
+                e[j] = exp2_fast(v);
+                s += e[j];
+                t = fmaf(e[j], fmaxf(v, kLowest), t);
             }
-            g = row_terms(a, row, weight, inv_w, za, m, s, t, true, sums);
+            // logits that are all NaN leave m at -inf and s NaN
+            g = row_terms(a, in, inv_w, go, za != neg_inf() && !(m == neg_inf() && s == 0.0f), fmaf(za, x.scale, x.shift), s, t, true, sums);
         }
         if (GRAD) {
 #pragma unroll
             for (int j = 0; j < AM; ++j) {
                 if (j < A && live) {
-                    const float u = z[j] - m;
-                    float d = exp2_fast(u * kLog2e) * g.inv_s * fmaf(g.ce, fmaxf(u, kLowest), g.k) + (j == action ? g.c1 : 0.0f);
-                    if (g.inv_s == 0.0f || z[j] == neg_inf()) d = 0.0f;
-                    rows_lds[me * A + j] = static_cast<T>(d * go);
+                    float d = grad_of(g, fmaf(z[j], x.scale, x.shift), e[j]) + (j == action ? g.c1 : 0.0f);
+                    if (g.none || z[j] == neg_inf()) d = 0.0f;
+                    rows_lds[me * A + j] = static_cast<T>(d);
                 }
             }
             __syncthreads();
@@ -311,7 +403,7 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
         }
         __syncthreads();
     }
-    finish_sums(a, sums, part);
+    finish_sums(a, sums, parts);
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------
@@ -319,74 +411,126 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
 // for the gradient).  One pass: a wavefront's maximum, its sums relative to that, and, where several wavefronts share the row, one
 // exchange of (maximum, sums) through LDS.
 // -------------------------------------------------------------------------------------------------------------------------------
+// Bits of -inf, in every element of a 32-bit word.  Pieces are put together as words: element by element the compiler gives each 16-bit
+// value a register of its own.
+template <typename T> constexpr uint32_t kNegInf = 0xff800000u;
+template <> constexpr uint32_t kNegInf<__bf16> = 0xff80ff80u;
+template <> constexpr uint32_t kNegInf<_Float16> = 0xfc00fc00u;
+
 template <typename T>
-__device__ __forceinline__ Chunk<T> load_chunk(const PolicyLossArgs &a, const T *row_ptr, long long row, int c) {
+__device__ __forceinline__ u32x4 rest_of_row(const T *row_ptr, int j0, int n) {
+    u32x4 raw;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t v = kNegInf<T>;
+        if (sizeof(T) == 4) {
+            if (j0 + w < n) v = reinterpret_cast<const uint32_t *>(row_ptr)[j0 + w];
+        } else {
+            if (j0 + 2 * w < n) v = (v & 0xffff0000u) | reinterpret_cast<const uint16_t *>(row_ptr)[j0 + 2 * w];
+            if (j0 + 2 * w + 1 < n) v = (v & 0xffffu) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row_ptr)[j0 + 2 * w + 1]) << 16;
+        }
+        raw[w] = v;
+    }
+    return raw;
+}
+
+// Piece c = lane + first of a row: the row's own address and `first` are the same for all lanes, the rest is 32 bits.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_values(const PolicyLossArgs &a, const T *row_ptr, int first, int lane) {
     constexpr int V = Chunk<T>::V;
     typedef typename Unaligned<sizeof(T)>::type U;
     Chunk<T> x;
+    if ((first + lane + 1) * V <= a.n_actions)
+        x.raw = *reinterpret_cast<const U *>(reinterpret_cast<const char *>(row_ptr + static_cast<long long>(first) * V) + static_cast<uint32_t>(lane) * 16u);
+    else
+        x.raw = rest_of_row(row_ptr, (first + lane) * V, a.n_actions);
+    return x;
+}
+
+// Unavailable actions become -inf.
+template <typename T>
+__device__ __forceinline__ void take_out(const PolicyLossArgs &a, Chunk<T> &x, long long row, int c) {
+    constexpr int V = Chunk<T>::V;
     const int j0 = c * V;
-    if (j0 + V <= a.n_actions) {
-        x.raw = *reinterpret_cast<const U *>(row_ptr + j0);
-    } else {
+    const long long at = row * a.avail_stride + j0;
+    uint32_t may = 0;                                      // a bit per element
+    if (a.avail_u8) {
+        const uint8_t *src = static_cast<const uint8_t *>(a.avail) + at;
+        if (j0 + V <= a.n_actions) {
+            uint32_t words[V / 4];
+            __builtin_memcpy(words, src, V);
 #pragma unroll
-        for (int i = 0; i < V; ++i) x.e[i] = j0 + i < a.n_actions ? row_ptr[j0 + i] : static_cast<T>(neg_inf());
-    }
-    if (a.avail && j0 + V <= a.n_actions) {
-        if (a.avail_u8) {
-            const uint8_t *may = static_cast<const uint8_t *>(a.avail) + row * a.avail_stride + j0;
-            uint8_t bytes[V];
-            __builtin_memcpy(bytes, may, V);
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (bytes[i] == 0) x.e[i] = static_cast<T>(neg_inf());
+            for (int i = 0; i < V; ++i) may |= (words[i / 4] >> (8 * (i & 3)) & 0xff) != 0 ? 1u << i : 0;
         } else {
-            const float *may = static_cast<const float *>(a.avail) + row * a.avail_stride + j0;
+            for (int i = 0; i < V && j0 + i < a.n_actions; ++i) may |= src[i] != 0 ? 1u << i : 0;
+        }
+    } else {
+        const float *src = static_cast<const float *>(a.avail) + at;
+        if (j0 + V <= a.n_actions) {
 #pragma unroll
             for (int q = 0; q < V / 4; ++q) {
-                const u32x4 four = reinterpret_cast<const u32x4_a4 *>(may)[q];
+                const u32x4 four = reinterpret_cast<const u32x4_a4 *>(src)[q];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if ((four[i] << 1) == 0) x.e[q * 4 + i] = static_cast<T>(neg_inf());        // +0 or -0
+                for (int i = 0; i < 4; ++i) may |= (four[i] << 1) != 0 ? 1u << (q * 4 + i) : 0;         // +0 and -0 are 0
             }
-        }
-    } else if (a.avail) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (j0 + i < a.n_actions) {
-                const long long at = row * a.avail_stride + j0 + i;
-                const bool may = a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[at] != 0 : static_cast<const float *>(a.avail)[at] != 0.0f;
-                if (!may) x.e[i] = static_cast<T>(neg_inf());
-            }
+        } else {
+            for (int i = 0; i < V && j0 + i < a.n_actions; ++i) may |= src[i] != 0.0f ? 1u << i : 0;
         }
     }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (sizeof(T) == 4) {
+            x.raw[w] = may >> w & 1 ? x.raw[w] : kNegInf<T>;
+        } else {
+            const uint32_t keep = (may >> (2 * w) & 1 ? 0xffffu : 0u) | (may >> (2 * w + 1) & 1 ? 0xffff0000u : 0u);
+            x.raw[w] = (x.raw[w] & keep) | (kNegInf<T> & ~keep);
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const PolicyLossArgs &a, const T *row_ptr, long long row, int c) {
+    Chunk<T> x = load_values<T>(a, row_ptr, 0, c);
+    if (a.avail) take_out<T>(a, x, row, c);
     return x;
 }
 
 template <typename T>
-__device__ __forceinline__ void store_grad(const PolicyLossArgs &a, long long row, int c, const Chunk<T> &x) {
+__device__ __forceinline__ void store_grad(const PolicyLossArgs &a, T *row_ptr, int first, int lane, const Chunk<T> &x) {
     constexpr int V = Chunk<T>::V;
     typedef typename Unaligned<sizeof(T)>::type U;
-    T *dst = static_cast<T *>(a.grad) + row * a.n_actions + c * V;
-    if (c * V + V <= a.n_actions) {
-        *reinterpret_cast<U *>(dst) = x.raw;
+    const int j0 = (first + lane) * V;
+    if (j0 + V <= a.n_actions) {
+        *reinterpret_cast<U *>(reinterpret_cast<char *>(row_ptr + static_cast<long long>(first) * V) + static_cast<uint32_t>(lane) * 16u) = x.raw;
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (c * V + i < a.n_actions) dst[i] = x.e[i];
+            if (j0 + i < a.n_actions) row_ptr[j0 + i] = x.e[i];
     }
 }
 
+// `nan`: the row's sums are not numbers, and 0 times them is not what a masked place gets
 template <typename T>
-__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, float m, const RowGrad &g, float go) {
+__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, const Exponent &ex, const RowGrad &g, bool nan) {
+    constexpr int V = Chunk<T>::V;
     Chunk<T> y;
+    float d[V];
 #pragma unroll
-    for (int i = 0; i < Chunk<T>::V; ++i) {
-        const float z = static_cast<float>(x.e[i]);
-        const float u = z - m;
-        float d = exp2_fast(u * kLog2e) * g.inv_s * fmaf(g.ce, fmaxf(u, kLowest), g.k) + (c * Chunk<T>::V + i == action ? g.c1 : 0.0f);
-        if (z == neg_inf()) d = 0.0f;
-        y.e[i] = static_cast<T>(d * go);
+    for (int i = 0; i < V; ++i) {
+        const float v = fmaf(static_cast<float>(x.e[i]), ex.scale, ex.shift);
+        d[i] = grad_of(g, v, exp2_fast(v));
     }
+    if (action / V == c) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] += c * V + i == action ? g.c1 : 0.0f;
+    }
+    if (nan) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (static_cast<float>(x.e[i]) == neg_inf()) d[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) y.e[i] = static_cast<T>(d[i]);
     return y;
 }
 
@@ -405,65 +549,102 @@ __device__ __forceinline__ float lanes_sum(float x) {
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_sums(const Chunk<T> &x, float base, float &s, float &t) {
+__device__ __forceinline__ void chunk_sums(const Chunk<T> &x, const Exponent &ex, float &s, float &t) {
 #pragma unroll
     for (int i = 0; i < Chunk<T>::V; ++i) {
-        const float u = static_cast<float>(x.e[i]) - base, e = exp2_fast(u * kLog2e);
+        const float v = fmaf(static_cast<float>(x.e[i]), ex.scale, ex.shift), e = exp2_fast(v);
         s += e;
-        t = fmaf(e, fmaxf(u, kLowest), t);
+        t = fmaf(e, fmaxf(v, kLowest), t);
     }
 }
 
+// s and t relative to the largest logit m, taken over to a larger one.  Without a possible action so far they are 0 -- or NaN, which
+// has to reach the result.
+__device__ __forceinline__ void rebase(float m, float to, float &s, float &t) {
+    if (m == neg_inf()) return;
+    const float d = fmaxf((m - to) * kLog2e, kLowest), f = exp2_fast(d);
+    t = f * fmaf(s, d, t);
+    s *= f;
+}
+
+// The pieces stay in registers as they were loaded: without this the compiler keeps the converted values and the exponentials of one
+// sweep for the next, twice to four times the registers, and three workgroups' worth of loads in flight become one.
+template <typename T>
+__device__ __forceinline__ void forget(Chunk<T> &x) { asm volatile("" : "+v"(x.raw)); }
+
 template <typename T, int L, int C, bool GRAD>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void oc_policy_loss_group_kernel(const PolicyLossArgs a) {
+__global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_eu(C >= 16 ? 4 : 1))) void oc_policy_loss_group_kernel(const PolicyLossArgs a) {
     constexpr int B = L < 256 ? 256 : L;                   // threads of a block
     constexpr int R = B / L;                               // rows of a block
     constexpr int LW = L < 64 ? L : 64;                    // lanes of a wavefront that share a row
     constexpr int NW = L / LW;                             // wavefronts that share a row
     constexpr int V = Chunk<T>::V;
     __shared__ float merge[2][NW][4];
-    __shared__ double part[B / 64];
+    __shared__ double part[B / 64], parts[B / 64][kSums];
     const float inv_w = GRAD ? inverse_weight(a, part) : 0.0f;
     const float go = GRAD ? a.grad_scale * (a.grad_out ? *a.grad_out : 1.0f) : 0.0f;
-    const int lane = threadIdx.x % L;
+    const int lane_of_row = threadIdx.x % L;
     const int n_chunks = (a.n_actions + V - 1) / V;
-    RowSums sums;
+    __shared__ RowSums group_sums[R];
+    // a row's addresses and scalars are the wavefront's, in scalar registers, where no two rows share one
+    const int group = L < 64 ? threadIdx.x / L : L < B ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : 0;
+    RowSums &sums = group_sums[group];
+    if (lane_of_row == 0) sums = RowSums{};
     int parity = 0;
-    for (long long row = static_cast<long long>(blockIdx.x) * R + threadIdx.x / L; row < a.rows; row += static_cast<long long>(gridDim.x) * R) {
+    for (long long row = static_cast<long long>(blockIdx.x) * R + group; row < a.rows; row += static_cast<long long>(gridDim.x) * R) {
+        // every row, and every sweep over it, computes its places anew: kept, the index of every element takes a register
+        int lane = lane_of_row;
+        asm volatile("" : "+v"(lane));
         const int action = action_of(a, row);
-        const float weight = action < 0 ? 0.0f : a.weights ? a.weights[row] : 1.0f;
-        if (weight == 0.0f) {
+        const RowInputs in = row_inputs(a, row, 0, action);
+        T *const grad_ptr = static_cast<T *>(a.grad) + row * a.n_actions;
+        if (in.weight == 0.0f) {
             if (GRAD) {
                 Chunk<T> zero;
                 zero.raw = u32x4{0, 0, 0, 0};
-                for (int c = lane; c < n_chunks; c += L) store_grad<T>(a, row, c, zero);
+                for (int c = lane; c < n_chunks; c += L) store_grad<T>(a, grad_ptr, 0, c, zero);
             }
             continue;
         }
         const T *row_ptr = static_cast<const T *>(a.logits) + row * a.row_stride;
         Chunk<T> x[C ? C : 1];
-        float m = neg_inf(), s = 0.0f, t = 0.0f;
         if (C) {
 #pragma unroll
             for (int i = 0; i < C; ++i)
-                if (lane + i * L < n_chunks) x[i] = load_chunk<T>(a, row_ptr, row, lane + i * L);
+                if (lane + i * L < n_chunks) x[i] = load_values<T>(a, row_ptr, i * L, lane);
         }
+        float m = neg_inf(), s = 0.0f, t = 0.0f;
         float za = static_cast<float>(row_ptr[action]);
         if (a.avail) {
             const long long at = row * a.avail_stride + action;
             if (a.avail_u8 ? static_cast<const uint8_t *>(a.avail)[at] == 0 : static_cast<const float *>(a.avail)[at] == 0.0f) za = neg_inf();
         }
         if (C) {
+            if (a.avail) {
+                asm volatile("" : "+v"(lane));
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (lane + i * L < n_chunks) {
+                        take_out<T>(a, x[i], row, lane + i * L);
+                        forget(x[i]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 if (lane + i * L < n_chunks)
 #pragma unroll
                     for (int k = 0; k < V; ++k) m = fmaxf(m, static_cast<float>(x[i].e[k]));
+            asm volatile("" : "+v"(lane));
             m = lanes_max<LW>(m);
-            const float base = m == neg_inf() ? 0.0f : m;
+            const Exponent ex = exponent_of(m);
 #pragma unroll
             for (int i = 0; i < C; ++i)
-                if (lane + i * L < n_chunks) chunk_sums<T>(x[i], base, s, t);
+                if (lane + i * L < n_chunks) {
+                    forget(x[i]);
+                    chunk_sums<T>(x[i], ex, s, t);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         } else {
             // running maximum and sums of a lane, rescaled where a piece raises the maximum
             for (int c = lane; c < n_chunks; c += L) {
@@ -472,21 +653,13 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void oc_policy_loss_group_kernel
 #pragma unroll
                 for (int k = 0; k < V; ++k) mc = fmaxf(mc, static_cast<float>(y.e[k]));
                 if (mc > m) {
-                    if (m != neg_inf()) {
-                        const float f = exp2_fast((m - mc) * kLog2e);
-                        t = f * fmaf(s, m - mc, t);
-                        s *= f;
-                    }
+                    rebase(m, mc, s, t);
                     m = mc;
                 }
-                chunk_sums<T>(y, m == neg_inf() ? 0.0f : m, s, t);
+                chunk_sums<T>(y, exponent_of(m), s, t);
             }
             const float mw = lanes_max<LW>(m);
-            if (mw > m && m != neg_inf()) {
-                const float f = exp2_fast((m - mw) * kLog2e);
-                t = f * fmaf(s, m - mw, t);
-                s *= f;
-            }
+            if (mw > m) rebase(m, mw, s, t);
             m = mw;
         }
         s = lanes_sum<LW>(s);
@@ -502,39 +675,45 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void oc_policy_loss_group_kernel
             t = 0.0f;
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
-                const float mw = merge[parity][w][0], sw = merge[parity][w][1], tw = merge[parity][w][2];
-                // a wavefront without a possible action has sums of 0 (or NaN, which has to reach the result)
-                const float f = mw == neg_inf() ? 1.0f : exp2_fast((mw - mm) * kLog2e);
-                s = fmaf(f, sw, s);
-                t = fmaf(f, mw == neg_inf() ? tw : fmaf(sw, fmaxf(mw - mm, kLowest), tw), t);
+                float sw = merge[parity][w][1], tw = merge[parity][w][2];
+                rebase(merge[parity][w][0], mm, sw, tw);
+                s += sw;
+                t += tw;
             }
             m = mm;
             parity ^= 1;                                   // the next row's exchange does not overwrite one that is still read
         }
-        if (lane == 0) sums.weight += weight;
-        const RowGrad g = row_terms(a, row, weight, inv_w, za, m, s, t, lane == 0, sums);
+        if (lane == 0) sums.s[5] += in.weight;
+        const Exponent ex = exponent_of(m);
+        const bool possible = za != neg_inf() && !(m == neg_inf() && s == 0.0f);          // logits that are all NaN leave m at -inf and s NaN
+        const RowGrad g = row_terms(a, in, inv_w, go, possible, fmaf(za, ex.scale, ex.shift), s, t, lane == 0, sums);
         if (GRAD) {
-            const bool none = g.inv_s == 0.0f;
+            const bool nan = s != s;
+            asm volatile("" : "+v"(lane));
             if (C) {
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const int c = lane + i * L;
                     if (c < n_chunks) {
-                        Chunk<T> y = grad_chunk<T>(x[i], c, action, m, g, go);
-                        if (none) y.raw = u32x4{0, 0, 0, 0};
-                        store_grad<T>(a, row, c, y);
+                        forget(x[i]);
+                        Chunk<T> y = grad_chunk<T>(x[i], c, action, ex, g, nan);
+                        if (g.none) y.raw = u32x4{0, 0, 0, 0};
+                        store_grad<T>(a, grad_ptr, i * L, lane, y);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             } else {
                 for (int c = lane; c < n_chunks; c += L) {
-                    Chunk<T> y = grad_chunk<T>(load_chunk<T>(a, row_ptr, row, c), c, action, m, g, go);
-                    if (none) y.raw = u32x4{0, 0, 0, 0};
-                    store_grad<T>(a, row, c, y);
+                    Chunk<T> y = grad_chunk<T>(load_chunk<T>(a, row_ptr, row, c), c, action, ex, g, nan);
+                    if (g.none) y.raw = u32x4{0, 0, 0, 0};
+                    store_grad<T>(a, grad_ptr, 0, c, y);
                 }
             }
         }
     }
-    finish_sums(a, sums, part);
+    RowSums mine = {};
+    if (lane_of_row == 0) mine = sums;
+    finish_sums(a, mine, parts);
 }
 
 template <typename T, bool GRAD>
@@ -545,14 +724,23 @@ void launch_policy_loss(const PolicyLossArgs &a, hipStream_t s, int *blocks) {
         *blocks = static_cast<int>(std::min<long long>(most, (a.rows + rows_per_block - 1) / rows_per_block));
         return dim3(*blocks);
     };
-    if (A <= 4) oc_policy_loss_rows_kernel<T, 4, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
-    else if (A <= 8) oc_policy_loss_rows_kernel<T, 8, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
-    else if (A <= 16) oc_policy_loss_rows_kernel<T, 16, GRAD><<<grid(kRowTile, kMaxBlocks), 256, 0, s>>>(a);
+    // a row is held in registers up to 1024 lanes x 16 pieces: 64 K f32 or 128 K 16-bit actions
+    const dim3 tiles = a.rows <= 2 * kRowTile ? dim3(1) : grid(kRowTile, kMaxBlocks);           // two tiles: one block, no launch to join
+    if (a.rows <= 2 * kRowTile) *blocks = 1;
+    if (A <= 16) {
+        if (A <= 4) oc_policy_loss_rows_kernel<T, 4, false, GRAD><<<tiles, 256, 0, s>>>(a);
+        else if (A == 5) oc_policy_loss_rows_kernel<T, 5, true, GRAD><<<tiles, 256, 0, s>>>(a);
+        else if (A == 6) oc_policy_loss_rows_kernel<T, 6, true, GRAD><<<tiles, 256, 0, s>>>(a);
+        else if (A <= 8) oc_policy_loss_rows_kernel<T, 8, false, GRAD><<<tiles, 256, 0, s>>>(a);
+        else oc_policy_loss_rows_kernel<T, 16, false, GRAD><<<tiles, 256, 0, s>>>(a);
+    }
     else if (chunks <= 16) oc_policy_loss_group_kernel<T, 16, 1, GRAD><<<grid(16, kMaxBlocks), 256, 0, s>>>(a);
     else if (chunks <= 64) oc_policy_loss_group_kernel<T, 16, 4, GRAD><<<grid(16, kMaxBlocks), 256, 0, s>>>(a);
     else if (chunks <= 64 * 4) oc_policy_loss_group_kernel<T, 64, 4, GRAD><<<grid(4, kMaxBlocks), 256, 0, s>>>(a);
     else if (chunks <= 256 * 4) oc_policy_loss_group_kernel<T, 256, 4, GRAD><<<grid(1, kMaxBlocks), 256, 0, s>>>(a);
     else if (chunks <= 512 * 8) oc_policy_loss_group_kernel<T, 512, 8, GRAD><<<grid(1, kMaxBlocks), 512, 0, s>>>(a);
+    else if (chunks <= 512 * 16) oc_policy_loss_group_kernel<T, 512, 16, GRAD><<<grid(1, kMaxBlocks), 512, 0, s>>>(a);
+    else if (chunks <= 1024 * 16) oc_policy_loss_group_kernel<T, 1024, 16, GRAD><<<grid(1, kMaxBlocks), 1024, 0, s>>>(a);
     else oc_policy_loss_group_kernel<T, 1024, 0, GRAD><<<grid(1, kMaxBlocks), 1024, 0, s>>>(a);
 }
 
@@ -606,19 +794,18 @@ extern "C" int oc_policy_loss(const oc_policy_loss_args *p, int what, void *d_wo
     a.want_sums = what != OC_LOSS_BACKWARD;
     a.weight_from = what == OC_LOSS_FORWARD ? WEIGHT_NONE : what == OC_LOSS_BACKWARD ? WEIGHT_GIVEN : a.rows <= kSelfWeightRows ? WEIGHT_SELF : WEIGHT_PARTIALS;
     if (a.weight_from == WEIGHT_PARTIALS) {
-        a.n_weight_partials = static_cast<int>(std::min<long long>(kWeightBlocks, (a.rows + 255) / 256));
+        a.n_weight_partials = static_cast<int>(std::min<long long>(kWeightBlocks, (a.rows + 1023) / 1024));
         oc_policy_weight_kernel<<<dim3(a.n_weight_partials), 256, 0, s>>>(a);
     }
     int blocks = 0;
     // one block finishes by itself
-    const int rows_per_block = a.n_actions <= 16 ? kRowTile : 1;
-    a.finalize_here = a.rows <= rows_per_block;
+    a.finalize_here = a.rows <= (a.n_actions <= 16 ? 2 * kRowTile : 1);
     if (a.rows == 0) {
-        oc_policy_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, 0);
+        oc_policy_finalize_kernel<<<dim3(1), 1024, 0, s>>>(a, 0);
     } else {
         if (what == OC_LOSS_FORWARD) launch_policy_loss_type<false>(a, p->logits_type, s, &blocks);
         else launch_policy_loss_type<true>(a, p->logits_type, s, &blocks);
-        if (a.want_sums && !a.finalize_here) oc_policy_finalize_kernel<<<dim3(1), 256, 0, s>>>(a, blocks);
+        if (a.want_sums && !a.finalize_here) oc_policy_finalize_kernel<<<dim3(1), 1024, 0, s>>>(a, blocks);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_policy_loss: %s", hipGetErrorString(e));
