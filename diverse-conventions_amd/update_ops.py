@@ -6,6 +6,7 @@ allocator, keeps nothing between calls and never synchronises with the host.
 """
 import ctypes
 import math
+from array import array
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -259,6 +260,15 @@ def _one_piece(t):
     return True
 
 
+def _look_at(tensors, name, device):
+    """-> types, element counts, addresses of a list of tensors on one GPU"""
+    dtypes = {t.dtype for t in tensors}
+    if not tensors[0].is_cuda or set(map(torch.Tensor.get_device, tensors)) != {device.index} or not dtypes <= _TYPES.keys():
+        raise ValueError(f"{name} must be float32, bfloat16 or float16 CUDA tensors of one device")
+    types = [_TYPES[dtypes.pop()]] * len(tensors) if len(dtypes) == 1 else [_TYPES[t.dtype] for t in tensors]
+    return types, list(map(torch.Tensor.numel, tensors)), list(map(torch.Tensor.data_ptr, tensors))
+
+
 def clip_grad_norm(grads, max_norm=None, norm_type=2.0, out=None):
     """Norm of all elements of a list of gradient tensors, and clipping to it -- `torch.nn.utils.clip_grad_norm_` for the framework's
     updates (the reference: train/MAPPO/r_mappo.py before every optimiser step, `get_gard_norm` where it only logs):
@@ -267,41 +277,44 @@ def clip_grad_norm(grads, max_norm=None, norm_type=2.0, out=None):
 
     grads: f32 / bf16 / f16 CUDA tensors of one device, mixed as they come, each one dense piece of memory (any order of dimensions); or
     modules' parameters -- where an entry is an nn.Parameter its `.grad` is taken, and skipped if None.  max_norm None: the norm alone.
-    norm_type 2 or inf.  out: tensors of the same shapes, strides and types for the clipped gradients (default: in place; gradients that
+    norm_type 2 or inf.  out: tensors of the same shapes (contiguous ones: sizes), strides and types for the clipped gradients (default: in place; gradients that
     need no clipping are then not written).  The same tensor must not be listed twice.  -> norm, f32 scalar on the device; squares are
     added in f64, so no gradient is too small or too large for it."""
     if isinstance(grads, torch.Tensor):
         grads = [grads]
-    tensors = [g.grad if isinstance(g, torch.nn.Parameter) else g for g in grads]
+    plain = torch.Tensor                                 # hundreds of tensors: one cheap look at each property, all at once
+    tensors = [g if type(g) is plain else g.grad if isinstance(g, torch.nn.Parameter) else g for g in grads]
     tensors = [t for t in tensors if t is not None]
     if norm_type not in (2, 2.0, math.inf, "inf"):
         raise ValueError("norm_type must be 2 or inf")
     if max_norm is not None and not max_norm >= 0:
         raise ValueError("max_norm must not be negative")
+    if out is not None and (max_norm is None or len(out) != len(tensors)):
+        raise ValueError("out wants max_norm and one tensor per gradient")
     if not tensors:
         return torch.zeros((), dtype=torch.float32)
     n, device = len(tensors), tensors[0].device
-    types = [_TYPES.get(t.dtype, -1) for t in tensors]
-    if not tensors[0].is_cuda or {t.get_device() for t in tensors} != {device.index} or -1 in types:
-        raise ValueError("gradients must be float32, bfloat16 or float16 CUDA tensors of one device")
-    dense = [t.is_contiguous() for t in tensors]
-    for i, t in enumerate(tensors):
-        if not dense[i] and not _one_piece(t):
-            raise ValueError(f"gradient {i} is not one dense piece of memory")
-    counts, src, dst = [t.numel() for t in tensors], [t.data_ptr() for t in tensors], None
+    types, counts, src = _look_at(tensors, "gradients", device)
+    dense = all(map(plain.is_contiguous, tensors))
+    if not dense:
+        for i, t in enumerate(tensors):
+            if not _one_piece(t):
+                raise ValueError(f"gradient {i} is not one dense piece of memory")
     if max_norm is not None and len({p for p, c in zip(src, counts) if c}) != n - counts.count(0):
         raise ValueError("a gradient is listed twice")
+    dst = None
     if out is not None:
-        if max_norm is None or len(out) != n:
-            raise ValueError("out wants max_norm and one tensor per gradient")
-        for i, (o, t) in enumerate(zip(out, tensors)):
-            if o.dtype != t.dtype or o.get_device() != device.index or o.shape != t.shape or (o.stride() != t.stride() and not (dense[i] and o.is_contiguous())):
-                raise ValueError(f"out[{i}] must have the shape, strides, type and device of its gradient")
-        dst = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+        out_types, out_counts, dst = _look_at(out, "out", device)
+        if out_types != types or out_counts != counts:
+            raise ValueError("out must have the types and sizes of the gradients")
+        if not (dense and all(map(plain.is_contiguous, out))) and any(o.shape != t.shape or o.stride() != t.stride() for o, t in zip(out, tensors)):
+            raise ValueError("out must have the shapes and strides of the gradients")
+        dst = array("Q", dst)
     L = native.lib()
     workspace = torch.empty(L.oc_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    native.check(L.oc_grad_norm_clip(n, (ctypes.c_void_p * n)(*src), dst, (ctypes.c_int64 * n)(*counts), (ctypes.c_int32 * n)(*types),
-                                     -1.0 if max_norm is None else float(max_norm), 0 if norm_type in (2, 2.0) else 1, norm.data_ptr(),
-                                     workspace.data_ptr(), _stream(device)))
+    src, counts, types = array("Q", src), array("q", counts), array("i", types)
+    at = lambda a: None if a is None else a.buffer_info()[0]
+    native.check(L.oc_grad_norm_clip(n, at(src), at(dst), at(counts), at(types), -1.0 if max_norm is None else float(max_norm),
+                                     0 if norm_type in (2, 2.0) else 1, norm.data_ptr(), workspace.data_ptr(), _stream(device)))
     return norm
