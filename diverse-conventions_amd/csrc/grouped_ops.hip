@@ -67,23 +67,64 @@ template <> struct Mat<float> {
     }
 };
 
-// Place of 16-byte piece c of row r of a staged tile, in bytes.  Contiguous along the reduction: rows of 128 bytes, read by 16 lanes at 16
-// different rows at once.  Otherwise: rows of N elements, read at four rows 8 apart (16-bit: and four neighbours of each).  The exclusive
-// or spreads those over the banks.
-template <typename T, bool TR, int N>
-__device__ __forceinline__ int place(int r, int c) {
-    if (!TR) return r * 128 + ((c ^ (r & 7)) << 4);
+// Place of 16-byte piece c of row r of a staged tile, in bytes.  Contiguous along the reduction: rows of RB (64 or 128) bytes, read by 16
+// lanes at 16 different rows at once.  Otherwise: rows of N elements, read at four rows 8 apart (16-bit: and four neighbours of each).
+// The exclusive or spreads those over the banks; the piece at place p of row r is piece p under the same operation.
+template <typename T, bool TR, int N, int RB>
+__device__ __forceinline__ int swap_piece(int r, int c) {
+    if (!TR) return RB == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
     constexpr int kPieces = N * static_cast<int>(sizeof(T)) / 16;
-    if (sizeof(T) == 2) {
-        constexpr int kSegs = kPieces / 2;
-        const int h = ((r & 3) | (((r >> 3) & 3) << 2)) & (kSegs - 1);
-        return r * (kPieces * 16) + ((((c >> 1) ^ h) << 1 | (c & 1)) << 4);
-    }
-    return r * (kPieces * 16) + ((c ^ ((((r >> 2) & 3) << 2) & (kPieces - 1))) << 4);
+    if (sizeof(T) == 2) return c ^ ((((r & 3) | (((r >> 3) & 3) << 2)) & (kPieces / 2 - 1)) << 1);
+    return c ^ ((((r >> 2) & 3) << 2) & (kPieces - 1));
+}
+template <typename T, bool TR, int N, int RB>
+__device__ __forceinline__ int place(int r, int c) {
+    constexpr int kRow = TR ? N * static_cast<int>(sizeof(T)) : RB;
+    return r * kRow + (swap_piece<T, TR, N, RB>(r, c) << 4);
 }
 
-// A tile of one operand on its way from memory to LDS: every thread carries kPer pieces of 16 bytes.
-template <typename T, bool TR, int N, int THREADS, bool VEC>
+__device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];           // where pieces behind the reduction's end are read from
+
+// A tile of one operand, copied from memory to LDS without passing through registers (aligned rows): every thread asks for kPer pieces of
+// 16 bytes, a wavefront's 64 land one behind the other.  Indexes behind the operand's end are read from its last row or piece -- their
+// results are not stored --, reduction indexes behind the end from a piece of zeros, on both sides: what lies there may be anything.
+template <typename T, bool TR, int N, int RB, int THREADS>
+struct Copy {
+    static constexpr int V = 16 / sizeof(T), BK = RB / sizeof(T);
+    static constexpr int kRowPieces = TR ? N / V : RB / 16;
+    static constexpr int kPer = N * RB / 16 / THREADS;
+    static_assert(kPer * THREADS * 16 == N * RB, "every thread carries the same number of pieces");
+    const T *src[kPer];
+
+    __device__ __forceinline__ void init(const T *base, long long ld, long long at, long long r0, long long own) {
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int q = threadIdx.x + n * THREADS, row = q / kRowPieces, c = swap_piece<T, TR, N, RB>(row, q % kRowPieces);
+            const long long left = own - 1, i = TR ? c * V : row;
+            const long long mine = i <= left ? i : TR ? left / V * V : left;
+            src[n] = TR ? base + (r0 + row) * ld + at + mine : base + (at + mine) * ld + r0 + c * V;
+        }
+    }
+    // red: reduction indexes left from this step's first
+    __device__ __forceinline__ void issue(char *lds, long long ld, long long red) {
+        char *wave = lds + (threadIdx.x & ~63) * 16;
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const T *from = src[n];
+            if (red < BK) {
+                const int q = threadIdx.x + n * THREADS, row = q / kRowPieces;
+                const int r = TR ? row : swap_piece<T, TR, N, RB>(row, q % kRowPieces) * V;
+                if (r >= red) from = reinterpret_cast<const T *>(g_zero_piece);
+            }
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                             (__attribute__((address_space(3))) void *)(wave + n * THREADS * 16), 16, 0, 0);
+            src[n] += TR ? BK * ld : BK;
+        }
+    }
+};
+
+// The same through registers, for rows at any address and of any length: every thread carries kPer pieces of 16 bytes.
+template <typename T, bool TR, int N, int THREADS>
 struct Stage {
     static constexpr int V = 16 / sizeof(T), BK = 128 / sizeof(T);
     static constexpr int kRowPieces = TR ? N / V : 8;
@@ -108,9 +149,7 @@ struct Stage {
             const long long row_left = (TR ? red : own) - row, left = (TR ? own : red) - c * V;
             x[n] = u32x4{0, 0, 0, 0};
             if (row_left > 0 && left > 0) {
-                if (VEC) {
-                    x[n] = *reinterpret_cast<const u32x4 *>(src[n]);
-                } else if (left >= V) {
+                if (left >= V) {
                     x[n] = *reinterpret_cast<const u32x4_a2 *>(src[n]);
                 } else {
                     union { u32x4 raw; T e[V]; } p;
@@ -131,33 +170,66 @@ struct Stage {
 #pragma unroll
         for (int n = 0; n < kPer; ++n) {
             const int q = threadIdx.x + n * THREADS;
-            *reinterpret_cast<u32x4 *>(lds + place<T, TR, N>(q / kRowPieces, q % kRowPieces)) = x[n];
+            *reinterpret_cast<u32x4 *>(lds + place<T, TR, N, 128>(q / kRowPieces, q % kRowPieces)) = x[n];
         }
     }
 };
 
-// The lane's piece of an operand for matrix step kk (0, 1) of a staged tile: own index `own0 + lane % 16`, 16-bit: reduction indexes
-// 32 kk + 8 (lane / 16) + 0..7, f32: 16 kk + 4 (lane / 16) + 0..3.
-template <typename T, bool TR, int N>
-__device__ __forceinline__ typename Mat<T>::frag read_frag(const char *lds, int own0, int kk) {
+// The lanes' pieces of an operand for matrix step kk of a staged tile, COUNT own indexes 16 apart from `own0 + lane % 16` on; 16-bit:
+// reduction indexes 32 kk + 8 (lane / 16) + 0..7, f32: 16 kk + 4 (lane / 16) + 0..3.
+// The transposing reads are written out, four pieces and their wait at a time: in front of the builtin the compiler waits for every copy
+// to LDS that is on its way (it cannot tell that they go to other buffers), and there would be no pipeline.
+#define OC_READ_TR "ds_read_b64_tr_b16 "
+template <int STEP>
+__device__ __forceinline__ void read_transposed(uint64_t (&x)[2], uint32_t a) {
+    asm volatile(OC_READ_TR "%0, %2\n\t" OC_READ_TR "%1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x[0]), "=&v"(x[1]) : "v"(a), "n"(STEP) : "memory");
+}
+template <int STEP>
+__device__ __forceinline__ void read_transposed(uint64_t (&x)[4], uint32_t a, uint32_t b) {
+    asm volatile(OC_READ_TR "%0, %4\n\t" OC_READ_TR "%1, %4 offset:%6\n\t" OC_READ_TR "%2, %5\n\t" OC_READ_TR "%3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) : "v"(a), "v"(b), "n"(STEP) : "memory");
+}
+template <int STEP>
+__device__ __forceinline__ void read_transposed(uint64_t (&x)[8], uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile(OC_READ_TR "%0, %8\n\t" OC_READ_TR "%1, %8 offset:%12\n\t" OC_READ_TR "%2, %9\n\t" OC_READ_TR "%3, %9 offset:%12\n\t"
+                 OC_READ_TR "%4, %10\n\t" OC_READ_TR "%5, %10 offset:%12\n\t" OC_READ_TR "%6, %11\n\t" OC_READ_TR "%7, %11 offset:%12\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                 : "v"(a), "v"(b), "v"(c), "v"(d), "n"(STEP) : "memory");
+}
+#undef OC_READ_TR
+
+template <typename T, bool TR, int N, int RB, int COUNT>
+__device__ __forceinline__ void read_frags(const char *lds, int own0, int kk, typename Mat<T>::frag (&out)[COUNT]) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-    union { u32x4 raw; i16x4 half[2]; float f[4]; typename Mat<T>::frag v; } x;
-    if (!TR) {
-        x.raw = *reinterpret_cast<const u32x4 *>(lds + place<T, false, N>(own0 + i, g + 4 * kk));
-    } else if (sizeof(T) == 2) {
+    if constexpr (!TR) {
+#pragma unroll
+        for (int x = 0; x < COUNT; ++x) out[x] = *reinterpret_cast<const typename Mat<T>::frag *>(lds + place<T, false, N, RB>(own0 + 16 * x + i, g + 4 * kk));
+    } else if constexpr (sizeof(T) == 2) {
+        constexpr int kStep = 4 * N * 2;                   // reduction indexes 4 on: the same swizzle
+        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)lds));
         const int r = 32 * kk + 8 * g + (i >> 2);
-        const int at = place<T, true, N>(r, (own0 >> 4) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
-        constexpr int kRowBytes = N * 2;
-        x.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + at));
-        x.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + at + 4 * kRowBytes));     // rows 4 on: the same swizzle
+        const auto at = [&](int x) { return base + place<T, true, N, RB>(r, ((own0 >> 4) + x) * 2 + ((i & 3) >> 1)) + (i & 1) * 8; };
+        constexpr int kBatch = COUNT >= 4 ? 4 : COUNT;
+        static_assert(COUNT % kBatch == 0, "whole batches");
+#pragma unroll
+        for (int x = 0; x < COUNT; x += kBatch) {
+            union { uint64_t raw[2 * kBatch]; typename Mat<T>::frag v[kBatch]; } y;
+            if constexpr (kBatch == 4) read_transposed<kStep>(y.raw, at(x), at(x + 1), at(x + 2), at(x + 3));
+            else if constexpr (kBatch == 2) read_transposed<kStep>(y.raw, at(x), at(x + 1));
+            else read_transposed<kStep>(y.raw, at(x));
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) out[x + k] = y.v[k];
+        }
     } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int r = 16 * kk + 4 * g + s;
-            x.f[s] = *reinterpret_cast<const float *>(lds + place<T, true, N>(r, (own0 + i) >> 2) + ((own0 + i) & 3) * 4);
-        }
+        for (int x = 0; x < COUNT; ++x)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int r = 16 * kk + 4 * g + s, own = own0 + 16 * x + i;
+                out[x][s] = *reinterpret_cast<const float *>(lds + place<T, true, N, RB>(r, own >> 2) + (own & 3) * 4);
+            }
     }
-    return x.v;
 }
 
 // The workgroup's place in the run of its XCD: workgroups go round robin over 8 XCDs, each gets a contiguous run of `total` tiles.
@@ -169,9 +241,11 @@ __device__ __forceinline__ bool xcd_has(int block, int total) { return (block >>
 
 enum { PRODUCT_ROWS = 0, PRODUCT_WEIGHTS = 1 };
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, bool VEC, int PRODUCT>
+// RB: bytes of the reduction that a step takes per index of its own; STAGES: tiles in LDS, STAGES - 1 of them on their way (0: through
+// registers, two tiles).
+template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PRODUCT, int RB, int STAGES>
 __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(const GroupedArgs a) {
-    constexpr int THREADS = (BI / WI) * (BJ / WJ) * 64, BK = 128 / sizeof(T);
+    constexpr int THREADS = (BI / WI) * (BJ / WJ) * 64, BK = RB / sizeof(T);
     constexpr int FI = WI / 16, FJ = WJ / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -262,11 +336,50 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
 #pragma unroll
         for (int fj = 0; fj < FJ; ++fj) acc[fi][fj] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int wi = (wave % (BI / WI)) * WI, wj = (wave / (BI / WI)) * WJ;
-    constexpr int kBuffer = (BI + BJ) * 128, kJ = BI * 128;                 // two buffers, I's tile in front of J's
+    constexpr int kBuffer = (BI + BJ) * RB, kJ = BI * RB;                   // a buffer has I's tile in front of J's
     const int steps = red > 0 ? static_cast<int>((red + BK - 1) / BK) : 0;
-    if (steps > 0) {
-        Stage<T, TRI, BI, THREADS, VEC> si;
-        Stage<T, TRJ, BJ, THREADS, VEC> sj;
+    const auto multiply = [&](const char *li) {
+        const char *lj = li + kJ;
+#pragma unroll
+        for (int kk = 0; kk < RB / 64; ++kk) {
+            typename Mat<T>::frag fi[FI], fj[FJ];
+            read_frags<T, TRJ, BJ, RB>(lj, wj, kk, fj);
+            read_frags<T, TRI, BI, RB>(li, wi, kk, fi);
+#pragma unroll
+            for (int x = 0; x < FI; ++x)
+#pragma unroll
+                for (int y = 0; y < FJ; ++y) Mat<T>::mma(acc[x][y], fi[x], fj[y]);
+        }
+    };
+    if constexpr (STAGES > 0) {
+        Copy<T, TRI, BI, RB, THREADS> ci;
+        Copy<T, TRJ, BJ, RB, THREADS> cj;
+        constexpr int kLoads = ci.kPer + cj.kPer;          // of a wavefront and step
+        if (steps > 0) {
+            ci.init(base_i, a.ld_i, i0, r0, i_left);
+            cj.init(base_j, a.ld_j, j0, r0, j_left);
+        }
+        const auto issue = [&](int t) {
+            char *to = lds + t % STAGES * kBuffer;
+            const long long left = red - static_cast<long long>(t) * BK;
+            ci.issue(to, a.ld_i, left);
+            cj.issue(to + kJ, a.ld_j, left);
+        };
+        for (int t = 0; t < STAGES - 1 && t < steps; ++t) issue(t);
+        for (int t = 0; t < steps; ++t) {
+            // step t has arrived when at most the later ones are on their way; the barrier says so for the other wavefronts' parts, and
+            // that all are through with step t - 1, whose buffer the next copies go to
+            if (t + STAGES - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (t + STAGES - 1 < steps) issue(t + STAGES - 1);
+            multiply(lds + t % STAGES * kBuffer);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // this wavefront has read its part before it says so
+        }
+    } else if (steps > 0) {
+        Stage<T, TRI, BI, THREADS> si;
+        Stage<T, TRJ, BJ, THREADS> sj;
         si.init(base_i, a.ld_i, i0, r0);
         sj.init(base_j, a.ld_j, j0, r0);
         si.load(i_left, red);
@@ -283,19 +396,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
                 si.load(i_left, left);
                 sj.load(j_left, left);
             }
-            const char *li = lds + (t & 1) * kBuffer, *lj = li + kJ;
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                typename Mat<T>::frag fi[FI], fj[FJ];
-#pragma unroll
-                for (int x = 0; x < FI; ++x) fi[x] = read_frag<T, TRI, BI>(li, wi + 16 * x, kk);
-#pragma unroll
-                for (int x = 0; x < FJ; ++x) fj[x] = read_frag<T, TRJ, BJ>(lj, wj + 16 * x, kk);
-#pragma unroll
-                for (int x = 0; x < FI; ++x)
-#pragma unroll
-                    for (int y = 0; y < FJ; ++y) Mat<T>::mma(acc[x][y], fi[x], fj[y]);
-            }
+            multiply(lds + (t & 1) * kBuffer);
             if (more) {
                 char *next = lds + ((t + 1) & 1) * kBuffer;
                 si.store(next);
@@ -402,26 +503,26 @@ hipError_t launch_tiles(K kernel, int threads, int lds_bytes, long long blocks, 
     return hipGetLastError();
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PRODUCT>
-hipError_t launch_product(const GroupedArgs &a, bool vec, hipStream_t s) {
-    constexpr int threads = (BI / WI) * (BJ / WJ) * 64, lds = 2 * (BI + BJ) * 128;
+template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PRODUCT, int RB, int STAGES>
+hipError_t launch_product(const GroupedArgs &a, bool aligned, hipStream_t s) {
+    constexpr int threads = (BI / WI) * (BJ / WJ) * 64;
     const long long tiles_i = (a.ni + BI - 1) / BI;
     const long long blocks = PRODUCT == PRODUCT_ROWS ? (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i
                                                      : tiles_i * ((a.nj + BJ - 1) / BJ) * a.groups * a.splits;
-    return vec ? launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, true, PRODUCT>, threads, lds, blocks, a, s)
-               : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, false, PRODUCT>, threads, lds, blocks, a, s);
+    return aligned ? launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, RB, STAGES>, threads, STAGES * (BI + BJ) * RB, blocks, a, s)
+                   : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, 128, 0>, threads, 2 * (BI + BJ) * 128, blocks, a, s);
 }
 
 // Which tile: few rows a group -- narrow in rows, many workgroups, the weights stream through; enough work to fill the 256 CUs with
 // 256 x 256 tiles (16-bit types) -- those; else 128 x 128.
 template <typename T, bool TRI, bool TRJ>
-hipError_t launch_rows(const GroupedArgs &a, bool vec, hipStream_t s) {
-    if (a.rows <= 32LL * a.groups) return launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+hipError_t launch_rows(const GroupedArgs &a, bool aligned, hipStream_t s) {
+    if (a.rows <= 32LL * a.groups) return launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
     if constexpr (sizeof(T) == 2) {
-        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
     }
-    if (a.ni <= 64) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
-    return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS>(a, vec, s);
+    if (a.ni <= 64) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
+    return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
 }
 
 struct WeightPlan { int tile, splits, bias_splits; };
@@ -440,12 +541,12 @@ WeightPlan weight_plan(int type, long long rows, int groups, int ni, int nj) {
 }
 
 template <typename T>
-hipError_t launch_weights(const GroupedArgs &a, const WeightPlan &p, bool vec, hipStream_t s) {
+hipError_t launch_weights(const GroupedArgs &a, const WeightPlan &p, bool aligned, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS>(a, vec, s);
+        if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
     }
-    if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS>(a, vec, s);
-    return launch_product<T, 128, 128, 64, 64, true, true, PRODUCT_WEIGHTS>(a, vec, s);
+    if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS, 128, 3>(a, aligned, s);
+    return launch_product<T, 128, 128, 64, 64, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
 }
 
 template <typename T>
@@ -471,7 +572,7 @@ int check_grouped(const oc_grouped_linear_args *p, const char *who) {
 }
 
 template <typename T>
-hipError_t forward_type(const GroupedArgs &a, bool vec, hipStream_t s) { return launch_rows<T, false, false>(a, vec, s); }
+hipError_t forward_type(const GroupedArgs &a, bool aligned, hipStream_t s) { return launch_rows<T, false, false>(a, aligned, s); }
 
 template <typename T>
 hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &base, float *parts, hipStream_t s) {
@@ -528,10 +629,10 @@ extern "C" int oc_grouped_linear(const oc_grouped_linear_args *p, void *stream) 
     a.rows = p->rows; a.groups = p->groups; a.ni = p->out_features; a.red = p->in_features;
     a.offsets64 = p->offsets64 != 0; a.splits = 1;
     const int V = p->type == OC_F32 ? 4 : 8;
-    const bool vec = aligned_rows(p->d_weight, p->in_features, p->type) && aligned_rows(p->d_x, p->x_stride, p->type) && p->in_features % V == 0;
+    const bool aligned = aligned_rows(p->d_weight, p->in_features, p->type) && aligned_rows(p->d_x, p->x_stride, p->type) && p->in_features % V == 0;
     const OcDeviceScope on_device(oc_device_of_pointer(p->d_y));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t e = p->type == OC_F32 ? forward_type<float>(a, vec, s) : p->type == OC_BF16 ? forward_type<__bf16>(a, vec, s) : forward_type<_Float16>(a, vec, s);
+    const hipError_t e = p->type == OC_F32 ? forward_type<float>(a, aligned, s) : p->type == OC_BF16 ? forward_type<__bf16>(a, aligned, s) : forward_type<_Float16>(a, aligned, s);
     return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grouped_linear: %s", hipGetErrorString(e));
 }
 
