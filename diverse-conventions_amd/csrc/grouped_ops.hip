@@ -88,38 +88,44 @@ __device__ __attribute__((aligned(16))) uint32_t g_zero_piece[4];           // w
 // A tile of one operand, copied from memory to LDS without passing through registers (aligned rows): every thread asks for kPer pieces of
 // 16 bytes, a wavefront's 64 land one behind the other.  Indexes behind the operand's end are read from its last row or piece -- their
 // results are not stored --, reduction indexes behind the end from a piece of zeros, on both sides: what lies there may be anything.
+// What the lanes add to the tile's address is worked out once; the address itself moves in scalar registers (32 bits for the lanes: the host
+// takes the other way for rows beyond 2^31 bytes a tile).
 template <typename T, bool TR, int N, int RB, int THREADS>
 struct Copy {
     static constexpr int V = 16 / sizeof(T), BK = RB / sizeof(T);
     static constexpr int kRowPieces = TR ? N / V : RB / 16;
     static constexpr int kPer = N * RB / 16 / THREADS;
     static_assert(kPer * THREADS * 16 == N * RB, "every thread carries the same number of pieces");
-    const T *src[kPer];
+    uint32_t off[kPer];
+    const char *base;
+    long long step;
 
-    __device__ __forceinline__ void init(const T *base, long long ld, long long at, long long r0, long long own) {
+    __device__ __forceinline__ void init(const T *first, long long ld, long long at, long long r0, long long own) {
+        base = reinterpret_cast<const char *>(TR ? first + r0 * ld + at : first + at * ld + r0);
+        step = (TR ? BK * ld : BK) * static_cast<long long>(sizeof(T));
+        const int left = own > N ? N - 1 : static_cast<int>(own) - 1;
 #pragma unroll
         for (int n = 0; n < kPer; ++n) {
             const int q = threadIdx.x + n * THREADS, row = q / kRowPieces, c = swap_piece<T, TR, N, RB>(row, q % kRowPieces);
-            const long long left = own - 1, i = TR ? c * V : row;
-            const long long mine = i <= left ? i : TR ? left / V * V : left;
-            src[n] = TR ? base + (r0 + row) * ld + at + mine : base + (at + mine) * ld + r0 + c * V;
+            const int i = TR ? c * V : row, mine = i <= left ? i : TR ? left / V * V : left;
+            off[n] = static_cast<uint32_t>(TR ? row * ld + mine : mine * ld + c * V) * static_cast<uint32_t>(sizeof(T));
         }
     }
-    // red: reduction indexes left from this step's first
-    __device__ __forceinline__ void issue(char *lds, long long ld, long long red) {
-        char *wave = lds + (threadIdx.x & ~63) * 16;
+    // wave: the wavefront's number, red: reduction indexes left from this step's first
+    __device__ __forceinline__ void issue(char *lds, int wave, long long red) {
+        char *to = lds + wave * 1024;
 #pragma unroll
         for (int n = 0; n < kPer; ++n) {
-            const T *from = src[n];
+            const char *from = base + off[n];
             if (red < BK) {
                 const int q = threadIdx.x + n * THREADS, row = q / kRowPieces;
                 const int r = TR ? row : swap_piece<T, TR, N, RB>(row, q % kRowPieces) * V;
-                if (r >= red) from = reinterpret_cast<const T *>(g_zero_piece);
+                if (r >= red) from = reinterpret_cast<const char *>(g_zero_piece);
             }
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                             (__attribute__((address_space(3))) void *)(wave + n * THREADS * 16), 16, 0, 0);
-            src[n] += TR ? BK * ld : BK;
+                                             (__attribute__((address_space(3))) void *)(to + n * THREADS * 16), 16, 0, 0);
         }
+        base += step;
     }
 };
 
@@ -199,38 +205,55 @@ __device__ __forceinline__ void read_transposed(uint64_t (&x)[8], uint32_t a, ui
 }
 #undef OC_READ_TR
 
+// Places that do not change from step to step are kept in `off`.
 template <typename T, bool TR, int N, int RB, int COUNT>
-__device__ __forceinline__ void read_frags(const char *lds, int own0, int kk, typename Mat<T>::frag (&out)[COUNT]) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-    if constexpr (!TR) {
+struct Frags {
+    static constexpr int kOff = TR ? (sizeof(T) == 2 ? COUNT : 1) : RB / 64;
+    uint32_t off[kOff];
+
+    __device__ __forceinline__ void init(int own0) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+        if constexpr (!TR) {
 #pragma unroll
-        for (int x = 0; x < COUNT; ++x) out[x] = *reinterpret_cast<const typename Mat<T>::frag *>(lds + place<T, false, N, RB>(own0 + 16 * x + i, g + 4 * kk));
-    } else if constexpr (sizeof(T) == 2) {
-        constexpr int kStep = 4 * N * 2;                   // reduction indexes 4 on: the same swizzle
-        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)lds));
-        const int r = 32 * kk + 8 * g + (i >> 2);
-        const auto at = [&](int x) { return base + place<T, true, N, RB>(r, ((own0 >> 4) + x) * 2 + ((i & 3) >> 1)) + (i & 1) * 8; };
-        constexpr int kBatch = COUNT >= 4 ? 4 : COUNT;
-        static_assert(COUNT % kBatch == 0, "whole batches");
+            for (int kk = 0; kk < kOff; ++kk) off[kk] = place<T, false, N, RB>(own0 + i, g + 4 * kk);       // 16 rows on: the same swizzle
+        } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int x = 0; x < COUNT; x += kBatch) {
-            union { uint64_t raw[2 * kBatch]; typename Mat<T>::frag v[kBatch]; } y;
-            if constexpr (kBatch == 4) read_transposed<kStep>(y.raw, at(x), at(x + 1), at(x + 2), at(x + 3));
-            else if constexpr (kBatch == 2) read_transposed<kStep>(y.raw, at(x), at(x + 1));
-            else read_transposed<kStep>(y.raw, at(x));
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) out[x + k] = y.v[k];
+            for (int x = 0; x < COUNT; ++x) off[x] = place<T, true, N, RB>(8 * g + (i >> 2), ((own0 >> 4) + x) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+        } else {
+            off[0] = own0 + i;
         }
-    } else {
-#pragma unroll
-        for (int x = 0; x < COUNT; ++x)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int r = 16 * kk + 4 * g + s, own = own0 + 16 * x + i;
-                out[x][s] = *reinterpret_cast<const float *>(lds + place<T, true, N, RB>(r, own >> 2) + (own & 3) * 4);
-            }
     }
-}
+    // kk: the matrix step
+    __device__ __forceinline__ void read(const char *lds, int kk, typename Mat<T>::frag (&out)[COUNT]) const {
+        if constexpr (!TR) {
+#pragma unroll
+            for (int x = 0; x < COUNT; ++x) out[x] = *reinterpret_cast<const typename Mat<T>::frag *>(lds + off[kk] + x * 16 * RB);
+        } else if constexpr (sizeof(T) == 2) {
+            constexpr int kRow = N * 2, kStep = 4 * kRow;  // reduction indexes 4 on, and 32 on: the same swizzle
+            const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)lds)) + kk * 32 * kRow;
+            constexpr int kBatch = COUNT >= 4 ? 4 : COUNT;
+            static_assert(COUNT % kBatch == 0, "whole batches");
+#pragma unroll
+            for (int x = 0; x < COUNT; x += kBatch) {
+                union { uint64_t raw[2 * kBatch]; typename Mat<T>::frag v[kBatch]; } y;
+                if constexpr (kBatch == 4) read_transposed<kStep>(y.raw, base + off[x], base + off[x + 1], base + off[x + 2], base + off[x + 3]);
+                else if constexpr (kBatch == 2) read_transposed<kStep>(y.raw, base + off[x], base + off[x + 1]);
+                else read_transposed<kStep>(y.raw, base + off[x]);
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) out[x + k] = y.v[k];
+            }
+        } else {
+            const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+            for (int x = 0; x < COUNT; ++x)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int r = 16 * kk + 4 * g + s, own = off[0] + 16 * x;
+                    out[x][s] = *reinterpret_cast<const float *>(lds + place<T, true, N, RB>(r, own >> 2) + (own & 3) * 4);
+                }
+        }
+    }
+};
 
 // The workgroup's place in the run of its XCD: workgroups go round robin over 8 XCDs, each gets a contiguous run of `total` tiles.
 __device__ __forceinline__ int xcd_tile(int block, int total) {
@@ -248,7 +271,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     constexpr int THREADS = (BI / WI) * (BJ / WJ) * 64, BK = RB / sizeof(T);
     constexpr int FI = WI / 16, FJ = WJ / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_i = (a.ni + BI - 1) / BI;
     const T *base_i = static_cast<const T *>(a.I), *base_j = static_cast<const T *>(a.J);
     int it, group;
@@ -264,7 +287,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
             }
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off);
-            total += n;
+            total += __builtin_amdgcn_readfirstlane(n);
         }
         // rows of no group: before the first, behind the last
         const long long head = offset_at(a, 0), tail = offset_at(a, a.groups);
@@ -294,11 +317,11 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
             if (past) {
                 const int l = __ffsll(past) - 1;
                 group = b + l;
-                mine = __shfl(n, l);
-                before += __shfl(upto, l) - mine;
+                mine = __builtin_amdgcn_readlane(n, l);
+                before += __builtin_amdgcn_readlane(upto, l) - mine;
                 break;
             }
-            before += __shfl(upto, 63);
+            before += __builtin_amdgcn_readlane(upto, 63);
         }
         // the row tiles of a group go fastest: they share the weights' tile
         const int local = tile - before * tiles_i;
@@ -312,11 +335,11 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
         base_i += static_cast<long long>(group) * (TRI ? a.red : a.ni) * a.ld_i;
     } else {
         const int tiles_j = (a.nj + BJ - 1) / BJ, per_group = tiles_i * tiles_j;
-        int tile = xcd_tile(blockIdx.x, gridDim.x);
-        const int split = tile % a.splits;
-        tile /= a.splits;
-        group = tile / per_group;
-        const int local = tile % per_group;
+        // groups differ in rows: every XCD gets its share of each group, the same tiles of all of them
+        const int group_blocks = per_group * a.splits;
+        group = blockIdx.x / group_blocks;
+        const int in_group = xcd_tile(blockIdx.x - group * group_blocks, group_blocks);
+        const int split = in_group % a.splits, local = in_group / a.splits;
         it = local % tiles_i;
         j0 = static_cast<long long>(local / tiles_i) * BJ;
         j_left = a.nj - j0;
@@ -338,13 +361,17 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     const int wi = (wave % (BI / WI)) * WI, wj = (wave / (BI / WI)) * WJ;
     constexpr int kBuffer = (BI + BJ) * RB, kJ = BI * RB;                   // a buffer has I's tile in front of J's
     const int steps = red > 0 ? static_cast<int>((red + BK - 1) / BK) : 0;
+    Frags<T, TRI, BI, RB, FI> at_i;
+    Frags<T, TRJ, BJ, RB, FJ> at_j;
+    at_i.init(wi);
+    at_j.init(wj);
     const auto multiply = [&](const char *li) {
         const char *lj = li + kJ;
 #pragma unroll
         for (int kk = 0; kk < RB / 64; ++kk) {
             typename Mat<T>::frag fi[FI], fj[FJ];
-            read_frags<T, TRJ, BJ, RB>(lj, wj, kk, fj);
-            read_frags<T, TRI, BI, RB>(li, wi, kk, fi);
+            at_j.read(lj, kk, fj);
+            at_i.read(li, kk, fi);
 #pragma unroll
             for (int x = 0; x < FI; ++x)
 #pragma unroll
@@ -362,10 +389,49 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
         const auto issue = [&](int t) {
             char *to = lds + t % STAGES * kBuffer;
             const long long left = red - static_cast<long long>(t) * BK;
-            ci.issue(to, a.ld_i, left);
-            cj.issue(to + kJ, a.ld_j, left);
+            ci.issue(to, wave, left);
+            cj.issue(to + kJ, wave, left);
         };
         for (int t = 0; t < STAGES - 1 && t < steps; ++t) issue(t);
+        if constexpr (THREADS == 512) {
+            // Two wavefronts a SIMD, half a step apart: while one multiplies the other reads its pieces of the next step, so that LDS and
+            // the matrix unit work at the same time (side by side in the same phase they took turns: 2.8 times a step's matrix time).
+            // Barriers b0, b1, ..: wavefronts 0-3 read step t between b(2t-1) and b(2t), wavefronts 4-7 one barrier later.  Every wavefront
+            // has its copies of step t in LDS before b(2t-1), and the buffer of step t - 1 is read for the last time before it.
+            static_assert(RB == 64, "one matrix step");
+            if (steps > 0) {
+                if (steps >= STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                if (wave >= 4) __builtin_amdgcn_s_barrier();
+                for (int t = 0; t < steps; ++t) {
+                    const char *li = lds + t % STAGES * kBuffer;
+                    typename Mat<T>::frag fi[FI], fj[FJ];
+                    asm volatile("" ::: "memory");
+                    at_j.read(li + kJ, 0, fj);
+                    at_i.read(li, 0, fi);
+                    if (t + STAGES - 1 < steps) {
+                        issue(t + STAGES - 1);
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+                    } else {
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_barrier();
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                    for (int x = 0; x < FI; ++x)
+#pragma unroll
+                        for (int y = 0; y < FJ; ++y) Mat<T>::mma(acc[x][y], fi[x], fj[y]);
+                    __builtin_amdgcn_s_setprio(0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_barrier();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (wave < 4) __builtin_amdgcn_s_barrier();
+            }
+        } else
         for (int t = 0; t < steps; ++t) {
             // step t has arrived when at most the later ones are on their way; the barrier says so for the other wavefronts' parts, and
             // that all are through with step t - 1, whose buffer the next copies go to
@@ -558,7 +624,7 @@ hipError_t launch_join(const float *parts, void *out, long long n, int splits, h
 
 bool aligned_rows(const void *p, long long ld, int type) {
     const long long size = type == OC_F32 ? 4 : 2;
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && ld * size * 256 < 0x80000000LL;
 }
 
 int check_grouped(const oc_grouped_linear_args *p, const char *who) {
