@@ -386,11 +386,13 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
             ci.init(base_i, a.ld_i, i0, r0, i_left);
             cj.init(base_j, a.ld_j, j0, r0, j_left);
         }
+        int here = 0, there = 0;                           // the buffers of the step at hand and of the next one to be copied
+        const auto next = [](int at) { return at + kBuffer == STAGES * kBuffer ? 0 : at + kBuffer; };
         const auto issue = [&](int t) {
-            char *to = lds + t % STAGES * kBuffer;
             const long long left = red - static_cast<long long>(t) * BK;
-            ci.issue(to, wave, left);
-            cj.issue(to + kJ, wave, left);
+            ci.issue(lds + there, wave, left);
+            cj.issue(lds + there + kJ, wave, left);
+            there = next(there);
         };
         for (int t = 0; t < STAGES - 1 && t < steps; ++t) issue(t);
         if constexpr (THREADS == 512) {
@@ -405,7 +407,8 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
                 __builtin_amdgcn_s_barrier();
                 if (wave >= 4) __builtin_amdgcn_s_barrier();
                 for (int t = 0; t < steps; ++t) {
-                    const char *li = lds + t % STAGES * kBuffer;
+                    const char *li = lds + here;
+                    here = next(here);
                     typename Mat<T>::frag fi[FI], fj[FJ];
                     asm volatile("" ::: "memory");
                     at_j.read(li + kJ, 0, fj);
@@ -440,7 +443,8 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             if (t + STAGES - 1 < steps) issue(t + STAGES - 1);
-            multiply(lds + t % STAGES * kBuffer);
+            multiply(lds + here);
+            here = next(here);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // this wavefront has read its part before it says so
         }
     } else if (steps > 0) {
@@ -585,7 +589,7 @@ template <typename T, bool TRI, bool TRJ>
 hipError_t launch_rows(const GroupedArgs &a, bool aligned, hipStream_t s) {
     if (a.rows <= 32LL * a.groups) return launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
     if constexpr (sizeof(T) == 2) {
-        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
+        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 5>(a, aligned, s);
     }
     if (a.ni <= 64) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
     return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
@@ -609,7 +613,7 @@ WeightPlan weight_plan(int type, long long rows, int groups, int ni, int nj) {
 template <typename T>
 hipError_t launch_weights(const GroupedArgs &a, const WeightPlan &p, bool aligned, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
+        if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS, 64, 5>(a, aligned, s);
     }
     if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS, 128, 3>(a, aligned, s);
     return launch_product<T, 128, 128, 64, 64, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
