@@ -42,6 +42,8 @@ struct GroupedArgs {
     long long rows;                                        // of the whole batch
     int groups, ni, nj, red;                               // ni: output row length; rows product: red; dW: nj = output rows per group
     int offsets64, splits;
+    void *bias_out;                                        // dW: db or NULL, by further workgroups of the launch
+    int bias_splits, weight_blocks;
 };
 
 __device__ __forceinline__ long long offset_at(const GroupedArgs &a, int g) {
@@ -264,6 +266,45 @@ __device__ __forceinline__ bool xcd_has(int block, int total) { return (block >>
 
 enum { PRODUCT_ROWS = 0, PRODUCT_WEIGHTS = 1 };
 
+// Column sums of dY per group: a workgroup has 64 columns of one group and one split of its rows; 4 columns a thread.
+template <typename T, int THREADS>
+__device__ __forceinline__ void column_sums(const GroupedArgs &a, int block, float (*part)[64]) {
+    const int blocks_n = (a.nj + 63) / 64;
+    const int split = block % a.bias_splits, tile = block / a.bias_splits, group = tile / blocks_n;
+    const int c0 = (tile % blocks_n) * 64 + (threadIdx.x & 15) * 4, lane_row = threadIdx.x >> 4;
+    constexpr int kRows = THREADS / 16;
+    const long long row0 = offset_at(a, group);
+    long long rows = offset_at(a, group + 1) - row0;
+    if (rows < 0) rows = 0;
+    const long long len = (rows + a.bias_splits - 1) / a.bias_splits, first = split * len, last = first + len < rows ? first + len : rows;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const T *src = static_cast<const T *>(a.J);
+    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (c0 + 4 <= a.nj) {
+#pragma unroll 4
+        for (long long r = first + lane_row; r < last; r += kRows) {
+            const four_t v = *reinterpret_cast<const four_t *>(src + (row0 + r) * a.ld_j + c0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += static_cast<float>(v[k]);
+        }
+    } else {
+        for (long long r = first + lane_row; r < last; r += kRows)
+            for (int k = 0; k < 4; ++k)
+                if (c0 + k < a.nj) s[k] += static_cast<float>(src[(row0 + r) * a.ld_j + c0 + k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[lane_row][(threadIdx.x & 15) * 4 + k] = s[k];
+    __syncthreads();
+    const int c = (tile % blocks_n) * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && c < a.nj) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) sum += part[k][threadIdx.x];
+        if (a.bias_splits > 1) static_cast<float *>(a.bias_out)[(static_cast<long long>(split) * a.groups + group) * a.nj + c] = sum;
+        else static_cast<T *>(a.bias_out)[static_cast<long long>(group) * a.nj + c] = static_cast<T>(sum);
+    }
+}
+
 // RB: bytes of the reduction that a step takes per index of its own; STAGES: tiles in LDS, STAGES - 1 of them on their way (0: through
 // registers, two tiles).
 template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PRODUCT, int RB, int STAGES>
@@ -335,6 +376,10 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
         base_i += static_cast<long long>(group) * (TRI ? a.red : a.ni) * a.ld_i;
     } else {
         const int tiles_j = (a.nj + BJ - 1) / BJ, per_group = tiles_i * tiles_j;
+        if (blockIdx.x >= static_cast<unsigned>(a.weight_blocks)) {
+            column_sums<T, THREADS>(a, blockIdx.x - a.weight_blocks, reinterpret_cast<float (*)[64]>(lds));
+            return;
+        }
         // groups differ in rows: every XCD gets its share of each group, the same tiles of all of them
         const int group_blocks = per_group * a.splits;
         group = blockIdx.x / group_blocks;
@@ -512,52 +557,21 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     }
 }
 
-// out[e] = sum over the splits, in their order
+// out[e] = sum over the splits, in their order; two arrays in one launch: dW's parts and db's behind them
 template <typename T>
-__global__ __launch_bounds__(256) void oc_grouped_join_kernel(const float *parts, T *out, long long n, int splits) {
+__global__ __launch_bounds__(256) void oc_grouped_join_kernel(const float *parts_w, T *out_w, long long n_w, int splits_w, const float *parts_b, T *out_b,
+                                                              long long n_b, int splits_b) {
+    const long long n = n_w + n_b;
     for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < n; e += static_cast<long long>(gridDim.x) * 256) {
+        const bool w = e < n_w;
+        const float *src = w ? parts_w + e : parts_b + (e - n_w);
+        const long long stride = w ? n_w : n_b;
+        const int splits = w ? splits_w : splits_b;
         float s = 0.0f;
-        for (int k = 0; k < splits; ++k) s += parts[k * n + e];
-        out[e] = static_cast<T>(s);
-    }
-}
-
-// Column sums of dY per group: a block has 64 columns of one group and one split of its rows; 4 columns a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void oc_grouped_bias_kernel(const GroupedArgs a) {
-    __shared__ float part[16][64];
-    const int blocks_i = (a.ni + 63) / 64;
-    const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, group = tile / blocks_i;
-    const int c0 = (tile % blocks_i) * 64 + (threadIdx.x & 15) * 4, lane_row = threadIdx.x >> 4;
-    const long long row0 = offset_at(a, group);
-    long long rows = offset_at(a, group + 1) - row0;
-    if (rows < 0) rows = 0;
-    const long long len = (rows + a.splits - 1) / a.splits, first = split * len, last = first + len < rows ? first + len : rows;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const T *src = static_cast<const T *>(a.J);
-    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    if (c0 + 4 <= a.ni) {
-#pragma unroll 4
-        for (long long r = first + lane_row; r < last; r += 16) {
-            const four_t v = *reinterpret_cast<const four_t *>(src + (row0 + r) * a.ld_j + c0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] += static_cast<float>(v[k]);
-        }
-    } else {
-        for (long long r = first + lane_row; r < last; r += 16)
-            for (int k = 0; k < 4; ++k)
-                if (c0 + k < a.ni) s[k] += static_cast<float>(src[(row0 + r) * a.ld_j + c0 + k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) part[lane_row][(threadIdx.x & 15) * 4 + k] = s[k];
-    __syncthreads();
-    const int c = (tile % blocks_i) * 64 + threadIdx.x;
-    if (threadIdx.x < 64 && c < a.ni) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) sum += part[k][threadIdx.x];
-        if (a.splits > 1) static_cast<float *>(a.out)[(static_cast<long long>(split) * a.groups + group) * a.ni + c] = sum;
-        else static_cast<T *>(a.out)[static_cast<long long>(group) * a.ni + c] = static_cast<T>(sum);
+#pragma unroll 8
+        for (int k = 0; k < splits; ++k) s += src[k * stride];
+        if (w) out_w[e] = static_cast<T>(s);
+        else out_b[e - n_w] = static_cast<T>(s);
     }
 }
 
@@ -577,10 +591,16 @@ template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PR
 hipError_t launch_product(const GroupedArgs &a, bool aligned, hipStream_t s) {
     constexpr int threads = (BI / WI) * (BJ / WJ) * 64;
     const long long tiles_i = (a.ni + BI - 1) / BI;
-    const long long blocks = PRODUCT == PRODUCT_ROWS ? (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i
-                                                     : tiles_i * ((a.nj + BJ - 1) / BJ) * a.groups * a.splits;
-    return aligned ? launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, RB, STAGES>, threads, STAGES * (BI + BJ) * RB, blocks, a, s)
-                   : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, 128, 0>, threads, 2 * (BI + BJ) * 128, blocks, a, s);
+    long long blocks = (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i;
+    GroupedArgs b = a;
+    if (PRODUCT == PRODUCT_WEIGHTS) {
+        const long long weight_blocks = b.out ? tiles_i * ((a.nj + BJ - 1) / BJ) * a.groups * a.splits : 0;
+        blocks = weight_blocks + (b.bias_out ? static_cast<long long>((a.nj + 63) / 64) * a.groups * a.bias_splits : 0);
+        if (weight_blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+        b.weight_blocks = static_cast<int>(weight_blocks);
+    }
+    return aligned ? launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, RB, STAGES>, threads, STAGES * (BI + BJ) * RB, blocks, b, s)
+                   : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, 128, 0>, threads, 2 * (BI + BJ) * 128, blocks, b, s);
 }
 
 // Which tile: few rows a group -- narrow in rows, many workgroups, the weights stream through; enough work to fill the 256 CUs with
@@ -591,7 +611,7 @@ hipError_t launch_rows(const GroupedArgs &a, bool aligned, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 5>(a, aligned, s);
     }
-    if (a.ni <= 64) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
+    if (a.ni <= 64 || (sizeof(T) == 4 && a.ni <= 192)) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
     return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
 }
 
@@ -615,15 +635,8 @@ hipError_t launch_weights(const GroupedArgs &a, const WeightPlan &p, bool aligne
     if constexpr (sizeof(T) == 2) {
         if (p.tile == 256) return launch_product<T, 256, 256, 128, 64, true, true, PRODUCT_WEIGHTS, 64, 5>(a, aligned, s);
     }
-    if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS, 128, 3>(a, aligned, s);
+    if (p.tile == 64) return launch_product<T, 64, 64, 32, 32, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
     return launch_product<T, 128, 128, 64, 64, true, true, PRODUCT_WEIGHTS, 64, 4>(a, aligned, s);
-}
-
-template <typename T>
-hipError_t launch_join(const float *parts, void *out, long long n, int splits, hipStream_t s) {
-    const int blocks = static_cast<int>(std::min<long long>(4096, (n + 255) / 256));
-    oc_grouped_join_kernel<T><<<dim3(blocks), 256, 0, s>>>(parts, static_cast<T *>(out), n, splits);
-    return hipGetLastError();
 }
 
 bool aligned_rows(const void *p, long long ld, int type) {
@@ -657,25 +670,22 @@ hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &bas
         if (e != hipSuccess) return e;
     }
     const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
-    if (p->d_dweight) {
+    if (p->d_dweight || p->d_dbias) {
         GroupedArgs a = base;
         a.I = p->d_x; a.J = p->d_dy;
         a.ld_i = p->x_stride; a.ld_j = N; a.ld_out = K;
-        a.ni = K; a.nj = N; a.splits = plan.splits;
-        a.out = plan.splits > 1 ? static_cast<void *>(parts) : p->d_dweight;
+        a.ni = K; a.nj = N; a.splits = plan.splits; a.bias_splits = plan.bias_splits;
+        const long long n_w = p->d_dweight && plan.splits > 1 ? static_cast<long long>(p->groups) * N * K : 0;
+        const long long n_b = p->d_dbias && plan.bias_splits > 1 ? static_cast<long long>(p->groups) * N : 0;
+        float *const parts_b = parts + n_w * plan.splits;
+        a.out = n_w ? static_cast<void *>(parts) : p->d_dweight;
+        a.bias_out = n_b ? static_cast<void *>(parts_b) : p->d_dbias;
         e = launch_weights<T>(a, plan, aligned_rows(p->d_x, p->x_stride, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
-        const long long n = static_cast<long long>(p->groups) * N * K;
-        if (e == hipSuccess && plan.splits > 1) e = launch_join<T>(parts, p->d_dweight, n, plan.splits, s);
-        if (e != hipSuccess) return e;
-        parts += plan.splits > 1 ? plan.splits * n : 0;
-    }
-    if (p->d_dbias) {
-        GroupedArgs a = base;
-        a.J = p->d_dy; a.ld_j = N; a.ni = N; a.splits = plan.bias_splits;
-        a.out = plan.bias_splits > 1 ? static_cast<void *>(parts) : p->d_dbias;
-        oc_grouped_bias_kernel<T><<<dim3(static_cast<unsigned>((N + 63) / 64 * static_cast<long long>(p->groups) * plan.bias_splits)), 256, 0, s>>>(a);
-        e = hipGetLastError();
-        if (e == hipSuccess && plan.bias_splits > 1) e = launch_join<T>(parts, p->d_dbias, static_cast<long long>(p->groups) * N, plan.bias_splits, s);
+        if (e == hipSuccess && n_w + n_b) {
+            oc_grouped_join_kernel<T><<<dim3(static_cast<unsigned>(std::min<long long>(4096, (n_w + n_b + 255) / 256))), 256, 0, s>>>(
+                parts, static_cast<T *>(p->d_dweight), n_w, plan.splits, parts_b, static_cast<T *>(p->d_dbias), n_b, plan.bias_splits);
+            e = hipGetLastError();
+        }
     }
     return e;
 }
