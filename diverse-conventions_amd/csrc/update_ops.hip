@@ -775,6 +775,7 @@ extern "C" int oc_policy_loss(const oc_policy_loss_args *p, int what, void *d_wo
     if (reinterpret_cast<uintptr_t>(p->d_logits) % element || reinterpret_cast<uintptr_t>(p->d_grad) % element ||
         reinterpret_cast<uintptr_t>(p->d_weight) % 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
         return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: a pointer is not aligned to its elements (workspace: 8 bytes)");
+    if (p->n_actions > (1 << 28)) return oc_internal_fail(OC_ERR_UNSUPPORTED, "oc_policy_loss: n_actions %d beyond 2^28", p->n_actions);
     if (!(p->clip_param >= 0.0))
         return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_policy_loss: clip_param %g", p->clip_param);
     if (p->rows == 0 && what == OC_LOSS_BACKWARD) return OC_OK;

@@ -16,7 +16,7 @@ def _args(x, weight, offsets, bias):
     if not x.is_cuda or x.dtype not in _TYPES or x.dim() != 2:
         raise ValueError("x must be a float32, bfloat16 or float16 CUDA tensor [rows, in_features]")
     rows, k = x.shape
-    if weight.dim() != 3 or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous() or weight.shape[2] != k or 0 in weight.shape:
+    if weight.dim() != 3 or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous() or weight.shape[2] != k or 0 in weight.shape or max(weight.shape) >= 2 ** 31:
         raise ValueError(f"weight must be a contiguous {x.dtype} tensor [groups, out_features, {k}] on {x.device}")
     groups, n = weight.shape[:2]
     if bias is not None and (tuple(bias.shape) != (groups, n) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous()):
@@ -52,6 +52,7 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        # looked at again: hooks on saved tensors (checkpointing, keeping them on the host) may hand back others
         x, weight, offsets = ctx.saved_tensors
         want_x, want_w, _, want_b = ctx.needs_input_grad
         a = _args(x, weight, offsets, None)

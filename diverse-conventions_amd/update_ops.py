@@ -49,8 +49,8 @@ class _PolicyCall:
         if not logits.is_cuda or logits.dtype not in _TYPES or logits.dim() < 1:
             raise ValueError("logits must be a float32, bfloat16 or float16 CUDA tensor [..., actions]")
         n_actions = logits.shape[-1]
-        if not 1 <= n_actions < 2 ** 31:
-            raise ValueError("logits need at least one action")
+        if not 1 <= n_actions <= 2 ** 28:
+            raise ValueError("logits need 1 to 2^28 actions")
         rows = logits.numel() // n_actions
         dev = logits.device
         flat = logits if logits.dim() == 2 else logits.reshape(1, -1) if logits.dim() == 1 else logits.flatten(0, -2)
@@ -65,8 +65,7 @@ class _PolicyCall:
             ref = None                                   # no reference policy: no KL term
         else:
             ref = ref_log_probs
-        self.keep = [logits, actions, old_log_probs, advantages, ref, active_masks, available_actions]
-        self.shape, self.dtype, self.device, self.rows = logits.shape, logits.dtype, dev, rows
+        self.shape, self.dtype, self.device = logits.shape, logits.dtype, dev
         a = self.args = native.OcPolicyLossArgs()
         a.d_logits, a.d_actions = logits.data_ptr(), actions.data_ptr()
         a.d_old_log_probs = _rows_f32("old_log_probs", old_log_probs, rows, dev)
@@ -99,13 +98,6 @@ class _PolicyCall:
         native.check(native.lib().oc_policy_loss(ctypes.byref(a), _FORWARD_GRAD if want_grad else _FORWARD, workspace.data_ptr(), _stream(dev)))
         return loss, stats, grad
 
-    def backward(self, weight, grad_out):
-        a = self.args
-        grad = torch.empty(self.shape, dtype=self.dtype, device=self.device)
-        a.d_weight, a.d_grad, a.d_grad_out, a.grad_scale = weight.data_ptr(), grad.data_ptr(), grad_out.data_ptr(), 1.0
-        native.check(native.lib().oc_policy_loss(ctypes.byref(a), _BACKWARD, None, _stream(self.device)))
-        return grad
-
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
@@ -121,9 +113,13 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss, _):
+        # looked at again: hooks on saved tensors (checkpointing, keeping them on the host) may hand back others
         logits, actions, old, adv, ref, masks, avail = ctx.saved_tensors
-        call = _PolicyCall(logits, actions, old, adv, *ctx.coefs, ref, masks, avail)
-        grad = call.backward(ctx.weight, grad_loss.to(torch.float32).contiguous())
+        a = _PolicyCall(logits, actions, old, adv, *ctx.coefs, ref, masks, avail).args
+        grad_loss = grad_loss.to(torch.float32).contiguous()
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        a.d_weight, a.d_grad, a.d_grad_out = ctx.weight.data_ptr(), grad.data_ptr(), grad_loss.data_ptr()
+        native.check(native.lib().oc_policy_loss(ctypes.byref(a), _BACKWARD, None, _stream(grad.device)))
         return (grad,) + (None,) * 9
 
 
@@ -189,19 +185,13 @@ class _ValueCall:
         native.check(native.lib().oc_value_loss(ctypes.byref(a), _FORWARD_GRAD if want_grad else _FORWARD, workspace.data_ptr(), _stream(dev)))
         return loss, grad
 
-    def backward(self, weight, grad_out):
-        a, dev = self.args, self.values.device
-        grad = torch.empty(self.values.shape, dtype=self.values.dtype, device=dev)
-        a.d_weight, a.d_grad, a.d_grad_out, a.grad_scale = weight.data_ptr(), grad.data_ptr(), grad_out.data_ptr(), 1.0
-        native.check(native.lib().oc_value_loss(ctypes.byref(a), _BACKWARD, None, _stream(dev)))
-        return grad
-
 
 class _ValueLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, values, preds, returns, masks, clip_param, huber_delta, norm):
         ctx.weight = torch.empty(1, dtype=torch.float64, device=values.device)
-        loss, _ = _ValueCall(values, preds, returns, clip_param, huber_delta, masks, norm).forward(False, weight=ctx.weight)
+        call = _ValueCall(values, preds, returns, clip_param, huber_delta, masks, norm)
+        loss, _ = call.forward(False, weight=ctx.weight)
         ctx.save_for_backward(values, preds, returns, masks)
         ctx.rest = (clip_param, huber_delta, norm)
         return loss
@@ -211,8 +201,12 @@ class _ValueLoss(torch.autograd.Function):
     def backward(ctx, grad_loss):
         values, preds, returns, masks = ctx.saved_tensors
         clip_param, huber_delta, norm = ctx.rest
-        call = _ValueCall(values, preds, returns, clip_param, huber_delta, masks, norm)
-        return (call.backward(ctx.weight, grad_loss.to(torch.float32).contiguous()),) + (None,) * 6
+        a = _ValueCall(values, preds, returns, clip_param, huber_delta, masks, norm).args
+        grad_loss = grad_loss.to(torch.float32).contiguous()
+        grad = torch.empty(values.shape, dtype=values.dtype, device=values.device)
+        a.d_weight, a.d_grad, a.d_grad_out = ctx.weight.data_ptr(), grad.data_ptr(), grad_loss.data_ptr()
+        native.check(native.lib().oc_value_loss(ctypes.byref(a), _BACKWARD, None, _stream(grad.device)))
+        return (grad,) + (None,) * 6
 
 
 def _normalizer(value_normalizer):

@@ -249,3 +249,51 @@ def test_a_population_of_critics_learns_in_one_pass():
     assert abs(float(norm) - float(want)) < 1e-3 * float(want)
     for a, b in zip(one, two):
         assert float((a.grad.double() - b.grad).norm()) < 1e-2 * float(b.grad.norm())
+
+
+@pytest.mark.gpu
+def test_grouped_linear_under_hooks_on_saved_tensors():
+    from diverse_conventions_amd import grouped_linear
+    x, w, b, dy, cuts = inputs([30, 20], 24, 40, "f32", 9, True)
+    offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    got = []
+    for hooked in (True, False):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        wide = torch.cat([leaves[0], leaves[0]], 1)
+        with torch.autograd.graph.save_on_cpu() if hooked else torch.enable_grad():
+            y = grouped_linear(wide[:, :24], leaves[1] * 1.0, offsets, leaves[2])
+        del wide
+        junk = [torch.full((50, 48), float("nan"), device="cuda") for _ in range(20)]
+        got.append(torch.autograd.grad(y, leaves, dy))
+        del junk
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+def test_grouped_linear_beyond_32_bit_offsets():
+    """Weights of more than 2^31 elements, rows and results behind 2^31 elements: the last group against the same group alone."""
+    from diverse_conventions_amd import grouped_linear
+    k, n, groups = 1024, 2048, 1030                        # 2.16e9 weights
+    w = torch.zeros((groups, n, k), dtype=torch.bfloat16, device="cuda")
+    x, last, _, dy, _ = inputs([40], k, n, "bf16", 10, True)
+    w[-1] = last[0]
+    cuts = torch.zeros(groups + 1, dtype=torch.int64, device="cuda")
+    cuts[-1] = 40
+    y = grouped_linear(x, w, cuts)
+    one = torch.tensor([0, 40], device="cuda")
+    assert torch.equal(y, grouped_linear(x, last, one))
+    del w
+    rows = 1_100_000                                       # 2.25e9 results, 1.1e9 inputs
+    big = torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda")
+    big[-40:] = x
+    leaf, weight = big.requires_grad_(), last.clone().requires_grad_()
+    y = grouped_linear(leaf, weight, torch.tensor([rows - 40, rows], device="cuda"))
+    alone = [x.clone().requires_grad_(), last.clone().requires_grad_()]
+    z = grouped_linear(alone[0], alone[1], one)
+    assert torch.equal(y[-40:], z) and not y[:-40:9973].any() and not y[-41].any()
+    d = torch.zeros_like(y)
+    d[-40:] = dy
+    dx, dw = torch.autograd.grad(y, (leaf, weight), d)
+    zx, zw = torch.autograd.grad(z, alone, dy)
+    assert torch.equal(dx[-40:], zx) and torch.equal(dw, zw) and not dx[:-40:9973].any() and not dx[-41].any()
+    torch.cuda.empty_cache()

@@ -532,3 +532,57 @@ def test_one_update_of_an_actor_and_a_critic():
     for a, b in zip(*results):
         # f32 on both sides: 1e-4 of the largest element (sums of 500 terms of which each side rounds every one)
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max())), (a, b)
+
+
+@pytest.mark.gpu
+def test_losses_under_hooks_on_saved_tensors_and_in_place_changes():
+    """Tensors that a hook keeps on the host come back as others, elsewhere; one changed in place is noticed."""
+    from diverse_conventions_amd import policy_loss, value_loss
+    s = policy_inputs(8, 300, 6, device="cuda")
+    v, v0, ret, w = value_inputs(8, 300, torch.float32, True, None)
+    kw = dict(kl_coef=0.05, ref_log_probs=s["ref"], active_masks=s["weights"], available_actions=s["avail"])
+
+    def both(hooked):
+        z, y = torch.zeros((300, 9), device="cuda"), v.clone().requires_grad_()
+        z[:, 1:7] = s["logits"]
+        leaf = z.requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if hooked else torch.enable_grad():
+            one, _ = policy_loss((leaf * 1.0)[:, 1:7], s["actions"], s["old"], s["adv"], **kw)
+            two = value_loss(y * 1.0, v0, ret, active_masks=w)
+        junk = [torch.full((300, 9), math.nan, device="cuda") for _ in range(20)]       # what was freed is overwritten
+        grads = torch.autograd.grad(one + two, (leaf, y))
+        del junk
+        return grads
+
+    for a, b in zip(both(True), both(False)):
+        assert torch.equal(a, b)
+    mid = s["logits"].clone().requires_grad_() * 1.0
+    loss, _ = policy_loss(mid, s["actions"], s["old"], s["adv"])
+    mid.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    loss, stats = policy_loss(s["logits"].clone().requires_grad_(), s["actions"], s["old"], s["adv"])
+    loss += 1.0                                            # the results are the caller's
+    stats.mul_(0.0)
+    loss.backward()
+
+
+@pytest.mark.gpu
+def test_policy_loss_beyond_32_bit_offsets():
+    """Rows whose first element lies behind 2^31 elements, and 2^32 bytes of gradient: the last rows against the same rows alone."""
+    from diverse_conventions_amd import policy_loss_grad
+    n, rows = 70001, 30700                                 # 2.149e9 elements, 4.3 GB each of logits and gradient in bfloat16
+    assert n * rows > 2 ** 31
+    logits = torch.zeros((rows, n), dtype=torch.bfloat16, device="cuda")
+    s = policy_inputs(3, 4, n, torch.bfloat16, "none", False, False, "cuda")
+    logits[-4:] = s["logits"]
+    actions = torch.full((rows,), -1, device="cuda")       # padding, but for the last rows
+    actions[-4:] = s["actions"]
+    old, adv = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    old[-4:], adv[-4:] = s["old"], s["adv"]
+    loss, _, grad = policy_loss_grad(logits, actions, old, adv)
+    want, _, alone = policy_loss_grad(s["logits"], s["actions"], s["old"], s["adv"])
+    assert torch.equal(grad[-4:], alone) and not grad[:-4:997].any() and not grad[-5].any()
+    assert abs(float(loss) - float(want)) <= 1e-6 * abs(float(want))      # f64 sums in another order, rounded once
+    del logits, grad
+    torch.cuda.empty_cache()
