@@ -11,7 +11,14 @@
 //
 // Which rows belong to which group is read from the offsets on the device: a workgroup counts the row tiles of all groups, finds its
 // own, and leaves if there is none, so that ragged groups cost no host round trip and no tile crosses a group.  Tiles are dealt to the
-// eight XCDs in contiguous runs: workgroups that share a network's weights share an L2.
+// eight XCDs in contiguous runs: workgroups that share a network's weights share an L2.  (dW: every XCD gets its share of every group,
+// because a group's tiles cost what its rows are: 583 -> 387 us on ragged groups.)
+//
+// What bounds it (MI355X).  16-bit, 256 x 256 tiles: 4096^3 bf16 128 us = 1077 TFLOP/s (the library's product 1460); 16 ragged groups, 16 k
+// rows x 2048 x 4096: 352 us forward (the last round of tiles is half empty, a group's last tile too; even groups 304 us = 905 TFLOP/s).
+// Without the matrix instructions the even forward takes 258 us, without the copies 220: the copies from L2 into LDS (8.5 TB/s over all
+// CUs) bound it, more steps in flight (3, 4) or another order of the steps change nothing.  f32: 4096^3 1034 us = 133 TFLOP/s (library
+// 915).  One to three rows a group: the weights' bytes, 252 MB in 58 us = 4.3 TB/s.
 
 #include <hip/hip_runtime.h>
 
@@ -318,6 +325,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     int it, group;
     long long j0, j_left, r0, red;                         // first output row and how many are left, first reduction index and their number
     long long out_row;
+    bool first_split = true;
     if (PRODUCT == PRODUCT_ROWS) {
         int total = 0;                                     // row tiles of all groups
         for (int b = 0; b < a.groups; b += 64) {
@@ -334,12 +342,15 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
         const long long head = offset_at(a, 0), tail = offset_at(a, a.groups);
         const long long stray = (head + (a.rows - tail)) * a.ni;
         for (long long e = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; e < stray; e += static_cast<long long>(gridDim.x) * THREADS) {
-            const long long r = e / a.ni, row = r < head ? r : tail + (r - head);
-            static_cast<T *>(a.out)[row * a.ld_out + e % a.ni] = static_cast<T>(0.0f);
+            const long long r = e / a.ni, row = r < head ? r : tail + (r - head), at = row * a.ld_out + e % a.ni;
+            if (a.splits == 1) static_cast<T *>(a.out)[at] = static_cast<T>(0.0f);
+            else
+                for (int k = 0; k < a.splits; ++k) static_cast<float *>(a.out)[k * a.rows * a.ld_out + at] = 0.0f;
         }
         total *= tiles_i;
-        if (!xcd_has(blockIdx.x, total)) return;
-        const int tile = xcd_tile(blockIdx.x, total);
+        const int split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
+        if (!xcd_has(block, total)) return;
+        const int tile = xcd_tile(block, total);
         int before = 0, mine = 0;
         group = 0;
         for (int b = 0; b < a.groups; b += 64) {
@@ -370,9 +381,11 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
         const long long row0 = offset_at(a, group), rows = offset_at(a, group + 1) - row0;
         j0 = row0 + static_cast<long long>(local % mine) * BJ;
         j_left = row0 + rows - j0;
-        r0 = 0;
-        red = a.red;
-        out_row = j0;
+        const long long len = ((a.red + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+        r0 = split * len;
+        red = a.red - r0 < len ? a.red - r0 : len;
+        out_row = split * a.rows + j0;
+        first_split = split == 0;
         base_i += static_cast<long long>(group) * (TRI ? a.red : a.ni) * a.ld_i;
     } else {
         const int tiles_j = (a.nj + BJ - 1) / BJ, per_group = tiles_i * tiles_j;
@@ -525,7 +538,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     for (int fi = 0; fi < FI; ++fi) {
         const int i = wi + 16 * fi + 4 * (lane >> 4);
         float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (PRODUCT == PRODUCT_ROWS && a.bias) {
+        if (PRODUCT == PRODUCT_ROWS && a.bias && first_split) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 if (i + k < i_left) b[k] = static_cast<float>(static_cast<const T *>(a.bias)[static_cast<long long>(group) * a.ni + i0 + i + k]);
@@ -535,13 +548,16 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
             const int j = wj + 16 * fj + (lane & 15);
             if (j >= j_left || i >= i_left) continue;
             const long long at = (out_row + j) * a.ld_out + i0 + i;
-            if (PRODUCT == PRODUCT_WEIGHTS && a.splits > 1) {
+            if (a.splits > 1) {
                 float *dst = static_cast<float *>(a.out) + at;
                 typedef float four_t __attribute__((ext_vector_type(4), aligned(4)));
-                if (i + 4 <= i_left) *reinterpret_cast<four_t *>(dst) = acc[fi][fj];
+                four_t v = acc[fi][fj];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += b[k];
+                if (i + 4 <= i_left) *reinterpret_cast<four_t *>(dst) = v;
                 else
                     for (int k = 0; k < 4; ++k)
-                        if (i + k < i_left) dst[k] = acc[fi][fj][k];
+                        if (i + k < i_left) dst[k] = v[k];
             } else {
                 T *dst = static_cast<T *>(a.out) + at;
                 typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -591,7 +607,7 @@ template <typename T, int BI, int BJ, int WI, int WJ, bool TRI, bool TRJ, int PR
 hipError_t launch_product(const GroupedArgs &a, bool aligned, hipStream_t s) {
     constexpr int threads = (BI / WI) * (BJ / WJ) * 64;
     const long long tiles_i = (a.ni + BI - 1) / BI;
-    long long blocks = (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i;
+    long long blocks = (a.rows / BJ + std::min<long long>(a.groups, a.rows)) * tiles_i * a.splits;
     GroupedArgs b = a;
     if (PRODUCT == PRODUCT_WEIGHTS) {
         const long long weight_blocks = b.out ? tiles_i * ((a.nj + BJ - 1) / BJ) * a.groups * a.splits : 0;
@@ -603,21 +619,59 @@ hipError_t launch_product(const GroupedArgs &a, bool aligned, hipStream_t s) {
                    : launch_tiles(oc_grouped_kernel<T, BI, BJ, WI, WJ, TRI, TRJ, PRODUCT, 128, 0>, threads, 2 * (BI + BJ) * 128, blocks, b, s);
 }
 
-// Which tile: few rows a group -- narrow in rows, many workgroups, the weights stream through; enough work to fill the 256 CUs with
-// 256 x 256 tiles (16-bit types) -- those; else 128 x 128.
+// Which tile.  Few rows a group: narrow in rows, many workgroups, the weights stream through (32 networks of 2048 x 2048, bf16: 32 rows
+// each 42 us against 57 with 128 x 128, 48 rows 60 against 57; f32: 64 rows 188 against 283, 96 rows 266 against 270).  Enough work for
+// most of the 256 CUs with 256 x 256 tiles (16-bit types): those (K = 2048, bf16: 180 tiles 55 us against 72 with 128 x 128, 128 tiles 54
+// against 48).  Short output rows: 64 x 64, f32 also up to 192 (61 k rows of 192: 31 us against 36).  Else 128 x 128.
+// Few tiles and a long reduction: the reduction is cut, too, into pieces of 256 or more (f32: 128), and a second launch adds the f32 parts up.
+enum { TILE_64x32, TILE_64, TILE_128, TILE_256 };
+struct RowsPlan { int tile, splits; };
+
+RowsPlan rows_plan(int type, long long rows, int groups, int ni, int red) {
+    RowsPlan p;
+    const bool f32 = type == OC_F32;
+    int bi = 64, bj = 64;
+    if (rows <= (f32 ? 80LL : 32LL) * groups) { p.tile = TILE_64x32; bj = 32; }
+    else if (!f32 && ni > 128 && (rows / 256 + groups / 2) * ((ni + 255) / 256) >= 150) { p.tile = TILE_256; bi = bj = 256; }
+    else if (ni <= 64 || (f32 && ni <= 192)) p.tile = TILE_64;
+    else { p.tile = TILE_128; bi = bj = 128; }
+    const long long tiles = (rows / bj + std::min<long long>(groups, rows)) * ((ni + bi - 1) / bi);
+    p.splits = tiles < 1 || tiles > 128 ? 1 : static_cast<int>(std::max<long long>(1, std::min<long long>({256 / tiles, red / (f32 ? 128 : 256), 16})));
+    return p;
+}
+
+// f32 parts of a rows product, in elements
+long long rows_parts(const RowsPlan &p, long long rows, int ni) { return p.splits > 1 ? p.splits * rows * ni : 0; }
+
+template <typename T>
+hipError_t launch_join(const float *parts_w, void *out_w, long long n_w, int splits_w, const float *parts_b, void *out_b, long long n_b, int splits_b, hipStream_t s) {
+    if (n_w + n_b == 0) return hipSuccess;
+    oc_grouped_join_kernel<T><<<dim3(static_cast<unsigned>(std::min<long long>(4096, (n_w + n_b + 255) / 256))), 256, 0, s>>>(
+        parts_w, static_cast<T *>(out_w), n_w, splits_w, parts_b, static_cast<T *>(out_b), n_b, splits_b);
+    return hipGetLastError();
+}
+
+// `parts`: rows_parts() floats
 template <typename T, bool TRI, bool TRJ>
-hipError_t launch_rows(const GroupedArgs &a, bool aligned, hipStream_t s) {
-    if (a.rows <= 32LL * a.groups) return launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
+hipError_t launch_rows(GroupedArgs a, const RowsPlan &p, float *parts, bool aligned, hipStream_t s) {
+    void *const out = a.out;
+    a.splits = p.splits;
+    if (p.splits > 1) a.out = parts;
+    hipError_t e = hipSuccess;
+    if (p.tile == TILE_64x32) e = launch_product<T, 64, 32, 16, 32, TRI, TRJ, PRODUCT_ROWS, 128, 3>(a, aligned, s);
+    else if (p.tile == TILE_64) e = launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
+    else if (p.tile == TILE_128) e = launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
     if constexpr (sizeof(T) == 2) {
-        if (a.ni > 128 && (a.rows / 256 + a.groups / 2) * ((a.ni + 255) / 256) >= 224) return launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 5>(a, aligned, s);
+        if (p.tile == TILE_256) e = launch_product<T, 256, 256, 128, 64, TRI, TRJ, PRODUCT_ROWS, 64, 5>(a, aligned, s);
     }
-    if (a.ni <= 64 || (sizeof(T) == 4 && a.ni <= 192)) return launch_product<T, 64, 64, 32, 32, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
-    return launch_product<T, 128, 128, 64, 64, TRI, TRJ, PRODUCT_ROWS, 64, 4>(a, aligned, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    return launch_join<T>(parts, out, a.rows * a.ni, p.splits, nullptr, nullptr, 0, 1, s);
 }
 
 struct WeightPlan { int tile, splits, bias_splits; };
 
 // The tile of dW and into how many pieces its rows are cut so that there are workgroups for every CU (a piece has 128 rows or more).
+// 256 x 256 where they fill the CUs without cutting (bf16, 8192 rows: 192 tiles 101 us against 44 with 128 x 128, 256 tiles 76 against 85).
 WeightPlan weight_plan(int type, long long rows, int groups, int ni, int nj) {
     WeightPlan p;
     const auto tiles = [&](int b) { return static_cast<long long>((ni + b - 1) / b) * ((nj + b - 1) / b) * groups; };
@@ -655,9 +709,6 @@ int check_grouped(const oc_grouped_linear_args *p, const char *who) {
 }
 
 template <typename T>
-hipError_t forward_type(const GroupedArgs &a, bool aligned, hipStream_t s) { return launch_rows<T, false, false>(a, aligned, s); }
-
-template <typename T>
 hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &base, float *parts, hipStream_t s) {
     hipError_t e = hipSuccess;
     const int K = p->in_features, N = p->out_features, V = p->type == OC_F32 ? 4 : 8;
@@ -666,8 +717,10 @@ hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &bas
         a.I = p->d_weight; a.J = p->d_dy; a.out = p->d_dx;
         a.ld_i = K; a.ld_j = N; a.ld_out = K;
         a.ni = K; a.red = N;
-        e = launch_rows<T, true, false>(a, aligned_rows(p->d_weight, K, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
+        const RowsPlan plan = rows_plan(p->type, p->rows, p->groups, K, N);
+        e = launch_rows<T, true, false>(a, plan, parts, aligned_rows(p->d_weight, K, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
         if (e != hipSuccess) return e;
+        parts += rows_parts(plan, p->rows, K);
     }
     const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
     if (p->d_dweight || p->d_dbias) {
@@ -681,46 +734,57 @@ hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &bas
         a.out = n_w ? static_cast<void *>(parts) : p->d_dweight;
         a.bias_out = n_b ? static_cast<void *>(parts_b) : p->d_dbias;
         e = launch_weights<T>(a, plan, aligned_rows(p->d_x, p->x_stride, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
-        if (e == hipSuccess && n_w + n_b) {
-            oc_grouped_join_kernel<T><<<dim3(static_cast<unsigned>(std::min<long long>(4096, (n_w + n_b + 255) / 256))), 256, 0, s>>>(
-                parts, static_cast<T *>(p->d_dweight), n_w, plan.splits, parts_b, static_cast<T *>(p->d_dbias), n_b, plan.bias_splits);
-            e = hipGetLastError();
-        }
+        if (e == hipSuccess) e = launch_join<T>(parts, p->d_dweight, n_w, plan.splits, parts_b, p->d_dbias, n_b, plan.bias_splits, s);
     }
     return e;
 }
 
 }  // namespace
 
-extern "C" int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *p) {
+extern "C" int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *p, int backward) {
     if (check_grouped(p, "oc_grouped_linear_workspace_bytes") != OC_OK) return -1;
-    const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, p->in_features, p->out_features);
-    const long long out = static_cast<long long>(p->groups) * p->out_features;
-    return ((plan.splits > 1 ? plan.splits * out * p->in_features : 0) + (plan.bias_splits > 1 ? plan.bias_splits * out : 0)) * static_cast<long long>(sizeof(float));
+    const int K = p->in_features, N = p->out_features;
+    long long floats;
+    if (!backward) {
+        floats = rows_parts(rows_plan(p->type, p->rows, p->groups, N, K), p->rows, N);
+    } else {
+        const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
+        const long long out = static_cast<long long>(p->groups) * N;
+        floats = rows_parts(rows_plan(p->type, p->rows, p->groups, K, N), p->rows, K) + (plan.splits > 1 ? plan.splits * out * K : 0) +
+                 (plan.bias_splits > 1 ? plan.bias_splits * out : 0);
+    }
+    return floats * static_cast<long long>(sizeof(float));
 }
 
-extern "C" int oc_grouped_linear(const oc_grouped_linear_args *p, void *stream) {
+extern "C" int oc_grouped_linear(const oc_grouped_linear_args *p, void *d_workspace, void *stream) {
     if (const int rc = check_grouped(p, "oc_grouped_linear")) return rc;
     if (p->rows == 0) return OC_OK;
     if (!p->d_y) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear: d_y is NULL");
+    const RowsPlan plan = rows_plan(p->type, p->rows, p->groups, p->out_features, p->in_features);
+    if (plan.splits > 1 && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear: needs a workspace of %lld bytes",
+                                static_cast<long long>(oc_grouped_linear_workspace_bytes(p, 0)));
     GroupedArgs a = {};
     a.I = p->d_weight; a.J = p->d_x; a.bias = p->d_bias; a.out = p->d_y; a.offsets = p->d_offsets;
     a.ld_i = p->in_features; a.ld_j = p->x_stride; a.ld_out = p->out_features;
     a.rows = p->rows; a.groups = p->groups; a.ni = p->out_features; a.red = p->in_features;
-    a.offsets64 = p->offsets64 != 0; a.splits = 1;
+    a.offsets64 = p->offsets64 != 0;
     const int V = p->type == OC_F32 ? 4 : 8;
     const bool aligned = aligned_rows(p->d_weight, p->in_features, p->type) && aligned_rows(p->d_x, p->x_stride, p->type) && p->in_features % V == 0;
     const OcDeviceScope on_device(oc_device_of_pointer(p->d_y));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t e = p->type == OC_F32 ? forward_type<float>(a, aligned, s) : p->type == OC_BF16 ? forward_type<__bf16>(a, aligned, s) : forward_type<_Float16>(a, aligned, s);
+    float *parts = static_cast<float *>(d_workspace);
+    const hipError_t e = p->type == OC_F32    ? launch_rows<float, false, false>(a, plan, parts, aligned, s)
+                         : p->type == OC_BF16 ? launch_rows<__bf16, false, false>(a, plan, parts, aligned, s)
+                                              : launch_rows<_Float16, false, false>(a, plan, parts, aligned, s);
     return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grouped_linear: %s", hipGetErrorString(e));
 }
 
 extern "C" int oc_grouped_linear_backward(const oc_grouped_linear_args *p, void *d_workspace, void *stream) {
     if (const int rc = check_grouped(p, "oc_grouped_linear_backward")) return rc;
     if (p->rows > 0 && !p->d_dy) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: d_dy is NULL");
-    const int64_t need = oc_grouped_linear_workspace_bytes(p);
-    if (need > 0 && (p->d_dweight || p->d_dbias) && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
+    const int64_t need = oc_grouped_linear_workspace_bytes(p, 1);
+    if (need > 0 && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
         return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: needs a workspace of %lld bytes", static_cast<long long>(need));
     GroupedArgs a = {};
     a.offsets = p->d_offsets; a.rows = p->rows; a.groups = p->groups; a.offsets64 = p->offsets64 != 0; a.splits = 1;

@@ -280,8 +280,9 @@ __device__ __forceinline__ float grad_of(const RowGrad &g, float v, float e) { r
 
 // -------------------------------------------------------------------------------------------------------------------------------
 // Up to 16 actions: a thread has a whole row.  The block's 256 rows are one contiguous piece of memory; it is copied through LDS in
-// 16-byte pieces, because lanes that each load their own 24 bytes touch every line of the piece once per load.  AM: 4, 8 or 16 values
-// are held in registers.
+// 16-byte pieces, because lanes that each load their own 24 bytes touch every line of the piece once per load.  AM: so many values are
+// held in registers.  6.55 M rows of 6 f32 with gradient: 103 us (446 MB, 4.3 TB/s) and 14 us for the weights in front; 360 vector
+// instructions a row with library logarithm, exponential and division made it 204 us.
 // -------------------------------------------------------------------------------------------------------------------------------
 constexpr int kRowTile = 256;
 
@@ -409,7 +410,8 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
 // -------------------------------------------------------------------------------------------------------------------------------
 // More actions: L lanes have a row together, each C pieces of 16 bytes of it in registers (C = 0: more than fits, the row is read again
 // for the gradient).  One pass: a wavefront's maximum, its sums relative to that, and, where several wavefronts share the row, one
-// exchange of (maximum, sums) through LDS.
+// exchange of (maximum, sums) through LDS.  4096 rows of 32768 bf16 with gradient: 138 us, 3.9 TB/s, three quarters of a copy's rate: two
+// exponentials and 17 other vector instructions an element take 84 us of it and overlap with the memory in part.
 // -------------------------------------------------------------------------------------------------------------------------------
 // Bits of -inf, in every element of a 32-bit word.  Pieces are put together as words: element by element the compiler gives each 16-bit
 // value a register of its own.
@@ -724,7 +726,9 @@ void launch_policy_loss(const PolicyLossArgs &a, hipStream_t s, int *blocks) {
         *blocks = static_cast<int>(std::min<long long>(most, (a.rows + rows_per_block - 1) / rows_per_block));
         return dim3(*blocks);
     };
-    // a row is held in registers up to 1024 lanes x 16 pieces: 64 K f32 or 128 K 16-bit actions
+    // A row is held in registers up to 1024 lanes x 16 pieces: 64 K f32 or 128 K 16-bit actions.  Two rows or more a CU at once: 4096 pieces
+    // as 512 x 8 138 us, as 256 x 16 150 us (4096 x 32768 bf16); 6253 pieces as 512 x 16 102 us, as 1024 x 8, one row a CU, 129 us
+    // (1023 x 50021 f16, forward and backward).
     const dim3 tiles = a.rows <= 2 * kRowTile ? dim3(1) : grid(kRowTile, kMaxBlocks);           // two tiles: one block, no launch to join
     if (a.rows <= 2 * kRowTile) *blocks = 1;
     if (A <= 16) {
@@ -744,8 +748,9 @@ void launch_policy_loss(const PolicyLossArgs &a, hipStream_t s, int *blocks) {
     else oc_policy_loss_group_kernel<T, 1024, 0, GRAD><<<grid(1, kMaxBlocks), 1024, 0, s>>>(a);
 }
 
-// Few rows: every block adds the weights up itself (8 bytes a row out of L2) and saves the launch that does it.
-constexpr long long kSelfWeightRows = 8192;
+// Few rows: every block adds the weights up itself and saves the launch that does it (6 actions: 1000 rows the same, 4000 rows 19 us
+// against 15, 8000 rows 25 against 15).
+constexpr long long kSelfWeightRows = 1024;
 
 template <bool GRAD>
 void launch_policy_loss_type(const PolicyLossArgs &a, int type, hipStream_t s, int *blocks) {
@@ -816,7 +821,8 @@ extern "C" int oc_policy_loss(const oc_policy_loss_args *p, int what, void *d_wo
 // Clipped value loss and its gradient (train/MAPPO/r_mappo.py, cal_value_loss): per sample with target y = (return - mean) / std
 //   e0 = y - v,  e1 = y - (v0 + clamp(v - v0, -c, c)),  loss = max(h(e0), h(e1)),  h(e) = e^2 / 2, or Huber's with delta;
 //   d loss / d v = -h'(e0) where |v - v0| <= c or h(e0) >= h(e1), else 0 (the clamped branch does not move with v).
-// 12..16 bytes read and 4 written per sample, nothing used twice: four samples per lane in one load each.
+// 12..16 bytes read and 4 written per sample, nothing used twice: four samples per lane in one load each.  26.2 M f32 samples: forward
+// 91 us (4.6 TB/s), backward 100 us (5.2 TB/s, a copy's rate).
 // ======================================================================================================
 namespace {
 
@@ -963,6 +969,7 @@ extern "C" int oc_value_loss(const oc_value_loss_args *p, int what, void *d_work
     if (reinterpret_cast<uintptr_t>(p->d_values) % element || reinterpret_cast<uintptr_t>(p->d_grad) % element ||
         reinterpret_cast<uintptr_t>(p->d_weight) % 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
         return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: a pointer is not aligned to its elements (workspace: 8 bytes)");
+    if (!(p->std > 0.0f)) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_value_loss: std %g", static_cast<double>(p->std));
     if (p->n == 0 && what == OC_LOSS_BACKWARD) return OC_OK;
     ValueLossArgs a = {};
     a.values = p->d_values; a.preds = p->d_value_preds; a.returns = p->d_returns; a.weights = p->d_active_masks;
@@ -1002,14 +1009,17 @@ extern "C" int oc_value_loss(const oc_value_loss_args *p, int what, void *d_work
 // arguments of the first pass (no table to copy, nothing kept between calls), kTensors a launch; its blocks leave a note of the piece
 // that they read, and the second pass is one launch over all notes, last piece first: what the caches still hold is read from there.
 // The squares are added in f64: neither 1e-30 nor 1e30 leaves the range, and the order of the sums does not show.  The second pass adds
-// up the first one's partial sums in every block.
+// up the first one's partial sums in every block (many: a launch between them does).  566 M elements, bf16 among f32 (1.13 GB): 245 + 8 +
+// 411 us, 4.6 TB/s read, then 5.5 TB/s.
 // ======================================================================================================
 namespace {
 
 constexpr int kTensors = 120;                              // kernel arguments stay below 4 KB
 constexpr int kNormBlocks = 16384;                         // pieces that the elements are cut into, beside one per tensor: short ones, so that
-                                                           // the last round of blocks is short (4096 pieces: 275 us for 1.13 GB instead of 230)
-constexpr int kJoinHere = 1024;                            // up to so many partial sums every block of the second pass adds up by itself
+                                                           // the last round of blocks is short (4096 pieces: 275 us for 1.13 GB instead of 245)
+constexpr int kJoinHere = 1024;                            // up to so many partial sums every block of the second pass adds up by itself, which
+                                                           // saves a launch of 5 us where that is half of the call; 14900 in every block: 441 us
+                                                           // for the second pass instead of 411
 constexpr long long kPiece = 4096;                         // and their unit
 
 struct Piece {                                             // what a block of the first pass has read

@@ -34,11 +34,18 @@ def _args(x, weight, offsets, bias):
     return a
 
 
+def _workspace(a, backward, device):
+    """What the C ABI asks for, a fresh one for every call; None if nothing."""
+    size = native.lib().oc_grouped_linear_workspace_bytes(ctypes.byref(a), backward)
+    return torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+
+
 def _forward(x, weight, offsets, bias):
     a = _args(x, weight, offsets, bias)
     y = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=x.device)
     a.d_y = y.data_ptr()
-    native.check(native.lib().oc_grouped_linear(ctypes.byref(a), _raw_stream(x.device.index)))
+    workspace = _workspace(a, 0, x.device)
+    native.check(native.lib().oc_grouped_linear(ctypes.byref(a), workspace if workspace is None else workspace.data_ptr(), _raw_stream(x.device.index)))
     return y
 
 
@@ -61,10 +68,9 @@ class _GroupedLinear(torch.autograd.Function):
         dx, dw, db = new(*x.shape) if want_x else None, new(*weight.shape) if want_w else None, new(*weight.shape[:2]) if want_b else None
         a.d_dy = dy.data_ptr()
         a.d_dx, a.d_dweight, a.d_dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
-        L = native.lib()
-        size = L.oc_grouped_linear_workspace_bytes(ctypes.byref(a))
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
-        native.check(L.oc_grouped_linear_backward(ctypes.byref(a), None if workspace is None else workspace.data_ptr(), _raw_stream(x.device.index)))
+        workspace = _workspace(a, 1, x.device)
+        native.check(native.lib().oc_grouped_linear_backward(ctypes.byref(a), workspace if workspace is None else workspace.data_ptr(),
+                                                             _raw_stream(x.device.index)))
         return dx, dw, None, db
 
 

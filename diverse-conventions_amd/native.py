@@ -258,9 +258,9 @@ def lib():
     L.oc_grad_norm_workspace_bytes.restype = i64
     L.oc_grad_norm_clip.argtypes = [ctypes.c_int32, vp, vp, vp, vp, fp, i32, vp, vp, vp]
     pg = ctypes.POINTER(OcGroupedLinearArgs)
-    L.oc_grouped_linear_workspace_bytes.argtypes = [pg]
+    L.oc_grouped_linear_workspace_bytes.argtypes = [pg, i32]
     L.oc_grouped_linear_workspace_bytes.restype = i64
-    L.oc_grouped_linear.argtypes = [pg, vp]
+    L.oc_grouped_linear.argtypes = [pg, vp, vp]
     L.oc_grouped_linear_backward.argtypes = [pg, vp, vp]
     ps = ctypes.POINTER(OcPolicyShape)
     L.oc_policy_packed_bytes.argtypes = [ps]

@@ -61,17 +61,13 @@ class _PolicyCall:
             raise ValueError(f"actions must be a contiguous int32, int64 or float32 tensor of {rows} elements on {dev}")
         if not clip_param >= 0:
             raise ValueError("clip_param must not be negative")
-        if kl_coef != 0 and ref_log_probs is None:
-            ref = None                                   # no reference policy: no KL term
-        else:
-            ref = ref_log_probs
         self.shape, self.dtype, self.device = logits.shape, logits.dtype, dev
         a = self.args = native.OcPolicyLossArgs()
         a.d_logits, a.d_actions = logits.data_ptr(), actions.data_ptr()
         a.d_old_log_probs = _rows_f32("old_log_probs", old_log_probs, rows, dev)
         a.d_advantages = _rows_f32("advantages", advantages, rows, dev)
-        if ref is not None:
-            a.d_ref_log_probs = _rows_f32("ref_log_probs", ref, rows, dev)
+        if ref_log_probs is not None:
+            a.d_ref_log_probs = _rows_f32("ref_log_probs", ref_log_probs, rows, dev)
         if active_masks is not None:
             a.d_active_masks = _rows_f32("active_masks", active_masks, rows, dev)
         if available_actions is not None:
@@ -272,7 +268,8 @@ def clip_grad_norm(grads, max_norm=None, norm_type=2.0, out=None):
     grads: f32 / bf16 / f16 CUDA tensors of one device, mixed as they come, each one dense piece of memory (any order of dimensions); or
     modules' parameters -- where an entry is an nn.Parameter its `.grad` is taken, and skipped if None.  max_norm None: the norm alone.
     norm_type 2 or inf.  out: tensors of the same shapes (contiguous ones: sizes), strides and types for the clipped gradients (default: in place; gradients that
-    need no clipping are then not written).  The same tensor must not be listed twice.  -> norm, f32 scalar on the device; squares are
+    need no clipping are then not written; this goes past autograd's version counters).  The same
+    tensor must not be listed twice, and none may overlap another.  -> norm, f32 scalar on the device; squares are
     added in f64, so no gradient is too small or too large for it."""
     if isinstance(grads, torch.Tensor):
         grads = [grads]

@@ -106,7 +106,7 @@ int oc_policy_loss(const oc_policy_loss_args *args, int what, void *d_workspace,
 
 /* Clipped value loss and its gradient (R_MAPPO.cal_value_loss, train/MAPPO/r_mappo.py; huber_loss / mse_loss of train/MAPPO/utils/util.py):
  *   y = (return - mean) / std;  e0 = y - v;  e1 = y - (v0 + clamp(v - v0, -c, c));  loss = sum w max(h(e0), h(e1)) / sum w
- * with h Huber's of huber_delta (< 0: e^2 / 2); clip_param < 0: h(e0) alone.  The gradient is that of h(e0) where |v - v0| <= c or
+ * with h Huber's of huber_delta (< 0: e^2 / 2); clip_param < 0: h(e0) alone; std must be positive.  The gradient is that of h(e0) where |v - v0| <= c or
  * h(e0) >= h(e1), else 0.  Samples of weight 0 are left out whatever they hold; no weight at all gives a loss of 0.
  * Passes, d_loss, d_weight (the sum of w), grad_scale and workspace as oc_policy_loss. */
 typedef struct {
@@ -140,8 +140,9 @@ int oc_grad_norm_clip(int32_t n_tensors, const void *const *d_grads, void *const
  *   forward:   y[r] = x[r] weight[g]^T + bias[g]          for d_offsets[g] <= r < d_offsets[g + 1]; rows of no group are 0
  *   backward:  dx[r] = dy[r] weight[g];  dweight[g] = sum_r dy[r]^T x[r];  dbias[g] = sum_r dy[r]  (each left out where its pointer is NULL)
  * Products run on the matrix cores with f32 accumulation; results are rounded once.  d_offsets [groups + 1] must not decrease; entries
- * are clamped into [0, rows], a group may be empty (its gradients are 0).  dweight and dbias of few, long groups are summed in f32
- * pieces through the workspace (oc_grouped_linear_workspace_bytes, 0 if none is needed), in a fixed order. */
+ * are clamped into [0, rows], a group may be empty (its gradients are 0).  Sums over many rows (dweight, dbias) and products of few rows
+ * over many features are cut into f32 parts, which the workspace holds (oc_grouped_linear_workspace_bytes of the pass; 0 if none is needed,
+ * < 0 for wrong arguments) and which are added up in a fixed order. */
 typedef struct {
     const void *d_x;                   /* [rows] of in_features values, x_stride elements apart */
     const void *d_weight;              /* [groups][out_features][in_features] */
@@ -153,8 +154,8 @@ typedef struct {
     int64_t rows, x_stride;
     int32_t groups, in_features, out_features, type, offsets64;
 } oc_grouped_linear_args;
-int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *args);
-int oc_grouped_linear(const oc_grouped_linear_args *args, void *stream);
+int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *args, int backward);
+int oc_grouped_linear(const oc_grouped_linear_args *args, void *d_workspace, void *stream);
 int oc_grouped_linear_backward(const oc_grouped_linear_args *args, void *d_workspace, void *stream);
 
 /* ---- fused policy inference on the matrix cores --------------------------------------------

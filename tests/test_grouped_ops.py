@@ -153,12 +153,12 @@ def test_grouped_linear_refuses_on_the_host():
     with pytest.raises(ValueError):
         grouped_linear(torch.zeros((4, 4)), torch.zeros((1, 4, 4)), torch.tensor([0, 4]))
     L, a = native.lib(), native.OcGroupedLinearArgs()
-    assert L.oc_grouped_linear(None, None) == -1 and L.oc_grouped_linear_workspace_bytes(None) == -1
-    assert L.oc_grouped_linear(ctypes.byref(a), None) == -1 and "groups 0" in L.oc_last_error().decode()
+    assert L.oc_grouped_linear(None, None, None) == -1 and L.oc_grouped_linear_workspace_bytes(None, 0) == -1
+    assert L.oc_grouped_linear(ctypes.byref(a), None, None) == -1 and "groups 0" in L.oc_last_error().decode()
     a.groups, a.in_features, a.out_features, a.rows, a.x_stride = 2, 8, 8, 4, 7
-    assert L.oc_grouped_linear(ctypes.byref(a), None) == -1 and "x_stride 7" in L.oc_last_error().decode()
+    assert L.oc_grouped_linear(ctypes.byref(a), None, None) == -1 and "x_stride 7" in L.oc_last_error().decode()
     a.x_stride = 8
-    assert L.oc_grouped_linear(ctypes.byref(a), None) == -1 and "NULL" in L.oc_last_error().decode()
+    assert L.oc_grouped_linear(ctypes.byref(a), None, None) == -1 and "NULL" in L.oc_last_error().decode()
     assert L.oc_grouped_linear_backward(ctypes.byref(a), None, None) == -1
 
 
@@ -297,3 +297,48 @@ def test_grouped_linear_beyond_32_bit_offsets():
     zx, zw = torch.autograd.grad(z, alone, dy)
     assert torch.equal(dx[-40:], zx) and torch.equal(dw, zw) and not dx[:-40:9973].any() and not dx[-41].any()
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,k,n", [([20000, 19111, 1], 16, 256), ([20000, 19111, 1], 72, 256), ([39000], 104, 264), ([39000], 160, 256),
+                                       ([0, 1, 5, 40, 64, 65, 130, 200] * 2, 1024, 1024), ([9000, 0, 10001], 1024, 24), ([9000, 3, 10001], 1024, 136)],
+                         ids=lambda v: str(v) if isinstance(v, int) else f"{len(v)}g{sum(v)}")
+def test_grouped_linear_large_tiles_of_few_steps(sizes, k, n, dtype):
+    """Reductions of none to a few steps through the tiles whose pipeline is deeper than that: short rows, narrow results, groups of few rows."""
+    run_and_check(sizes, k, n, dtype, 11, True, tail=1)
+
+
+@pytest.mark.gpu
+def test_grouped_linear_large_tiles_in_a_graph():
+    from diverse_conventions_amd import grouped_linear
+    x, w, b, dy, cuts = inputs([1000, 2048, 1500], 768, 2560, "bf16", 12, False, tail=4)
+    o, leaves = torch.tensor(cuts, dtype=torch.int32, device="cuda"), [t.requires_grad_() for t in (x, w, b)]
+
+    def step():
+        y = grouped_linear(x, w, o, b)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for r in range(4):
+        with torch.no_grad():
+            x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = [t.clone() for t in held]
+        assert all(torch.equal(a, c) for a, c in zip(seen, step())), r
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("sizes,k,n", [([1], 4096, 64), ([3], 2000, 520), ([33, 0, 5], 1032, 1000), ([120], 4100, 200), ([50], 999, 2001), ([200, 90], 600, 70),
+                                       ([7], 64, 4096), ([100], 130, 2056)], ids=lambda v: str(v) if isinstance(v, int) else f"{len(v)}g{sum(v)}")
+def test_grouped_linear_few_rows_of_many_features(sizes, k, n, dtype):
+    """Products whose reduction is cut and joined: forward over in_features, dx over out_features; rows of no group, without and with a bias."""
+    run_and_check(sizes, k, n, dtype, 13, True, head=2, tail=3)
+    run_and_check(sizes, k, n, dtype, 14, True, bias=False)
+    run_and_check(sizes, k, n, dtype, 15, False)
