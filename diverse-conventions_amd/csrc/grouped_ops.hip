@@ -622,7 +622,8 @@ hipError_t launch_product(const GroupedArgs &a, bool aligned, hipStream_t s) {
 // Which tile.  Few rows a group: narrow in rows, many workgroups, the weights stream through (32 networks of 2048 x 2048, bf16: 32 rows
 // each 42 us against 57 with 128 x 128, 48 rows 60 against 57; f32: 64 rows 188 against 283, 96 rows 266 against 270).  Enough work for
 // most of the 256 CUs with 256 x 256 tiles (16-bit types): those (K = 2048, bf16: 180 tiles 55 us against 72 with 128 x 128, 128 tiles 54
-// against 48).  Short output rows: 64 x 64, f32 also up to 192 (61 k rows of 192: 31 us against 36).  Else 128 x 128.
+// against 48).  Short output rows: 64 x 64, f32 also up to 192 (61 k rows of 192: 31 us against 36); so are fewer than 128 tiles of
+// 128 x 128 (1000 x 1000 x 1000: bf16 14 us against 22, f32 33 against 38).  Else 128 x 128.
 // Few tiles and a long reduction: the reduction is cut, too, into pieces of 256 or more (f32: 128), and a second launch adds the f32 parts up.
 enum { TILE_64x32, TILE_64, TILE_128, TILE_256 };
 struct RowsPlan { int tile, splits; };
@@ -634,6 +635,7 @@ RowsPlan rows_plan(int type, long long rows, int groups, int ni, int red) {
     if (rows <= (f32 ? 80LL : 32LL) * groups) { p.tile = TILE_64x32; bj = 32; }
     else if (!f32 && ni > 128 && (rows / 256 + groups / 2) * ((ni + 255) / 256) >= 150) { p.tile = TILE_256; bi = bj = 256; }
     else if (ni <= 64 || (f32 && ni <= 192)) p.tile = TILE_64;
+    else if ((rows / 128 + std::min<long long>(groups, rows)) * ((ni + 127) / 128) < 128) p.tile = TILE_64;
     else { p.tile = TILE_128; bi = bj = 128; }
     const long long tiles = (rows / bj + std::min<long long>(groups, rows)) * ((ni + bi - 1) / bi);
     p.splits = tiles < 1 || tiles > 128 ? 1 : static_cast<int>(std::max<long long>(1, std::min<long long>({256 / tiles, red / (f32 ? 128 : 256), 16})));
