@@ -342,3 +342,18 @@ def test_grouped_linear_few_rows_of_many_features(sizes, k, n, dtype):
     run_and_check(sizes, k, n, dtype, 13, True, head=2, tail=3)
     run_and_check(sizes, k, n, dtype, 14, True, bias=False)
     run_and_check(sizes, k, n, dtype, 15, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_grouped_linear_one_gradient_at_a_time(dtype):
+    """Only x, only the weights or only the bias wants a gradient: the others are not computed, the workspace holds what is."""
+    from diverse_conventions_amd import grouped_linear
+    for sizes, k, n in (([3000, 0, 40], 24, 72), ([5], 2048, 600)):
+        x, w, b, dy, cuts = inputs(sizes, k, n, dtype, 16, True)
+        offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+        want = update_oracle.grouped_linear(f64(x), f64(w), cuts, f64(b), f64(dy))[1:]
+        for only in range(3):
+            args = [t.clone().requires_grad_() if i == only else t for i, t in enumerate((x, w, b))]
+            y = grouped_linear(args[0], args[1], offsets, args[2])
+            check(torch.autograd.grad(y, args[only], dy)[0], want[only], None, dtype, True, only)

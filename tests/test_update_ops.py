@@ -586,3 +586,55 @@ def test_policy_loss_beyond_32_bit_offsets():
     assert abs(float(loss) - float(want)) <= 1e-6 * abs(float(want))      # f64 sums in another order, rounded once
     del logits, grad
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_losses_of_unusual_but_allowed_calls():
+    """One row without a leading dimension, no rows, coefficients of zero, a clip of zero, a broadcast byte mask over many actions, a KL
+    statistic without its term, backward twice."""
+    from diverse_conventions_amd import policy_loss, policy_loss_grad, value_loss
+    s = policy_inputs(21, 1, 6, available="none", weights=False, device="cuda")
+    leaf = s["logits"][0].clone().requires_grad_()
+    loss, stats = policy_loss(leaf, s["actions"].squeeze(), s["old"].squeeze(), s["adv"].squeeze(), kl_coef=0.05, ref_log_probs=s["ref"])
+    first, second = (torch.autograd.grad(loss, leaf, retain_graph=True)[0] for _ in range(2))
+    assert first.shape == (6,) and torch.equal(first, second)
+    check_policy(s, (loss.detach(), stats, first.unsqueeze(0)))
+    for n in (6, 40):
+        none = torch.zeros((0, n), device="cuda", requires_grad=True)
+        e = torch.zeros(0, device="cuda")
+        loss, _ = policy_loss(none, e, e, e)
+        assert float(loss.detach()) == 0 and torch.autograd.grad(loss, none)[0].shape == (0, n)
+    for n in (6, 40, 3000):
+        s = policy_inputs(22, 50, n, available="none", device="cuda")
+        mask = torch.ones((1, n), dtype=torch.uint8, device="cuda")
+        mask[0, 1] = 0
+        s["actions"] = torch.where(s["actions"] == 1, 0, s["actions"])
+        s["avail"] = mask.expand(50, n)
+        for clip, ce, ck in ((0.0, 0.0, 0.0), (0.2, 0.3, 0.0), (0.2, 0.0, 0.7)):
+            # exp(lp - old) is not within 1e-3 of the clip's borders: old is drawn anew around the masked distribution
+            z = torch.where(s["avail"] != 0, s["logits"].double(), -math.inf)
+            lp = torch.log_softmax(z, 1).gather(1, s["actions"][:, None]).squeeze(1)
+            s["old"] = (lp - torch.where(torch.arange(50, device="cuda") % 2 == 0, 0.1, -0.3)).float()
+            r = policy_loss_grad(s["logits"], s["actions"], s["old"], s["adv"], clip_param=clip, entropy_coef=ce, kl_coef=ck, ref_log_probs=s["ref"],
+                                 active_masks=s["weights"], available_actions=s["avail"])
+            check_policy(s, r, clip=clip, entropy_coef=ce, kl_coef=ck)
+    v = torch.tensor(0.5, device="cuda", requires_grad=True)
+    loss = value_loss(v, torch.tensor(0.4, device="cuda"), torch.tensor(2.0, device="cuda"))
+    (g,) = torch.autograd.grad(loss, v)
+    assert g.shape == () and abs(float(loss.detach()) - 1.125) < 1e-6 and abs(float(g) + 1.5) < 1e-6
+    empty = torch.zeros((0, 1), device="cuda", requires_grad=True)
+    assert torch.autograd.grad(value_loss(empty, empty.detach(), empty.detach()), empty)[0].shape == (0, 1)
+
+
+@pytest.mark.gpu
+def test_clip_grad_norm_of_nothing_and_onto_itself():
+    from diverse_conventions_amd import clip_grad_norm
+    empty = [torch.zeros(0, device="cuda"), torch.zeros((0, 3), device="cuda")]
+    assert float(clip_grad_norm(empty)) == 0 and float(clip_grad_norm(empty, 1.0)) == 0
+    grads = make_grads([5000, 33], 4)
+    raw = [g.clone() for g in grads]
+    norm = clip_grad_norm((g for g in grads), 0.25, out=grads)          # a generator; the results onto the gradients themselves
+    check_clip(norm, grads, raw, 0.25)
+    untouched = [g.clone() for g in raw]
+    clip_grad_norm(untouched, 0.0)
+    assert not any(g.any() for g in untouched)
