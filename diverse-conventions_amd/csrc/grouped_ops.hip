@@ -14,11 +14,12 @@
 // eight XCDs in contiguous runs: workgroups that share a network's weights share an L2.  (dW: every XCD gets its share of every group,
 // because a group's tiles cost what its rows are: 583 -> 387 us on ragged groups.)
 //
-// What bounds it (MI355X).  16-bit, 256 x 256 tiles: 4096^3 bf16 128 us = 1077 TFLOP/s (the library's product 1460); 16 ragged groups, 16 k
-// rows x 2048 x 4096: 352 us forward (the last round of tiles is half empty, a group's last tile too; even groups 304 us = 905 TFLOP/s).
-// Without the matrix instructions the even forward takes 258 us, without the copies 220: the copies from L2 into LDS (8.5 TB/s over all
-// CUs) bound it, more steps in flight (3, 4) or another order of the steps change nothing.  f32: 4096^3 1034 us = 133 TFLOP/s (library
-// 915).  One to three rows a group: the weights' bytes, 252 MB in 58 us = 4.3 TB/s.
+// What bounds it (MI355X).  16-bit, 256 x 256 tiles: 4096^3 bf16 119 us = 1155 TFLOP/s (the library's product 1460); 16 ragged groups, 16 k
+// rows x 2048 x 4096: 323 us forward, 370 dx, 365 dw (the last round of tiles is half empty, a group's last tile too; even groups 300 us
+// forward = 917 TFLOP/s).  When the even forward took 304 us it took 258 without the matrix instructions, 220 without the copies and 295
+// without the LDS reads: the copies from L2 into LDS (8.5 TB/s over all CUs) and the wavefronts' meeting at two barriers a step bound it;
+// more steps in flight (3, 4), another order of the steps or cache hints on the copies change nothing.  f32: 4096^3 1034 us = 133 TFLOP/s
+// (library 915 us).  One to three rows a group: the weights' bytes, 252 MB in 58 us = 4.3 TB/s.
 
 #include <hip/hip_runtime.h>
 
