@@ -42,16 +42,11 @@ __device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// A row's logits as exponents of 2 relative to its largest, v = z scale + shift in one fma.  Scale is log2 e; a largest logit beyond
-// 1e38 (a row at the type's lowest value, say) would leave the range with it, but there two logits are equal or 1e31 apart, and any scale
-// keeps exp2(v) at 1 or 0.
-struct Exponent { float scale, shift; };
-__device__ __forceinline__ Exponent exponent_of(float m) {
-    Exponent x;
-    x.scale = fabsf(m) < 1e38f || m == __builtin_inff() ? kLog2e : 0x1p-20f;
-    x.shift = m == neg_inf() ? 0.0f : -m * x.scale;
-    return x;
-}
+// A row's logits as exponents of 2 relative to its largest, v = (z - m) log2 e: the difference first, so that v is 0 at the largest logit and
+// carries 2^-23 of itself wherever the row lies.  (One fma with -m log2 e as its addend leaves that product's rounding in every v: 2^v is inf
+// or 0 for a largest logit beyond 1e10 or so, and where wavefronts share a row each has another rounding.)
+__device__ __forceinline__ float base_of(float m) { return m == neg_inf() ? 0.0f : m; }       // no possible action: exponents of -inf, not NaN
+__device__ __forceinline__ float exponent_of(float z, float base) { return (z - base) * kLog2e; }
 
 constexpr int kMaxBlocks = 2048;                           // of a launch that leaves one set of partial sums per block
 constexpr int kWeightBlocks = 1024;                        // of the launch that adds up the weights
@@ -376,25 +371,25 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
             m = fmaxf(m, z[j]);
         }
         RowGrad g = {0.0f, 0.0f, 0.0f, true};
-        const Exponent x = exponent_of(m);
+        const float base = base_of(m);
         float e[AM], s = 0.0f, t = 0.0f;
         if (in.weight != 0.0f) {
             sums.s[5] += in.weight;
 #pragma unroll
             for (int j = 0; j < AM; ++j) {
-                const float v = fmaf(z[j], x.scale, x.shift);
+                const float v = exponent_of(z[j], base);
                 e[j] = exp2_fast(v);
                 s += e[j];
                 t = fmaf(e[j], fmaxf(v, kLowest), t);
             }
             // logits that are all NaN leave m at -inf and s NaN
-            g = row_terms(a, in, inv_w, go, za != neg_inf() && !(m == neg_inf() && s == 0.0f), fmaf(za, x.scale, x.shift), s, t, true, sums);
+            g = row_terms(a, in, inv_w, go, za != neg_inf() && !(m == neg_inf() && s == 0.0f), exponent_of(za, base), s, t, true, sums);
         }
         if (GRAD) {
 #pragma unroll
             for (int j = 0; j < AM; ++j) {
                 if (j < A && live) {
-                    float d = grad_of(g, fmaf(z[j], x.scale, x.shift), e[j]) + (j == action ? g.c1 : 0.0f);
+                    float d = grad_of(g, exponent_of(z[j], base), e[j]) + (j == action ? g.c1 : 0.0f);
                     if (g.none || z[j] == neg_inf()) d = 0.0f;
                     rows_lds[me * A + j] = static_cast<T>(d);
                 }
@@ -513,13 +508,13 @@ __device__ __forceinline__ void store_grad(const PolicyLossArgs &a, T *row_ptr, 
 
 // `nan`: the row's sums are not numbers, and 0 times them is not what a masked place gets
 template <typename T>
-__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, const Exponent &ex, const RowGrad &g, bool nan) {
+__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, float base, const RowGrad &g, bool nan) {
     constexpr int V = Chunk<T>::V;
     Chunk<T> y;
     float d[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float v = fmaf(static_cast<float>(x.e[i]), ex.scale, ex.shift);
+        const float v = exponent_of(static_cast<float>(x.e[i]), base);
         d[i] = grad_of(g, v, exp2_fast(v));
     }
     if (action / V == c) {
@@ -551,10 +546,10 @@ __device__ __forceinline__ float lanes_sum(float x) {
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_sums(const Chunk<T> &x, const Exponent &ex, float &s, float &t) {
+__device__ __forceinline__ void chunk_sums(const Chunk<T> &x, float base, float &s, float &t) {
 #pragma unroll
     for (int i = 0; i < Chunk<T>::V; ++i) {
-        const float v = fmaf(static_cast<float>(x.e[i]), ex.scale, ex.shift), e = exp2_fast(v);
+        const float v = exponent_of(static_cast<float>(x.e[i]), base), e = exp2_fast(v);
         s += e;
         t = fmaf(e, fmaxf(v, kLowest), t);
     }
@@ -639,12 +634,12 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
                     for (int k = 0; k < V; ++k) m = fmaxf(m, static_cast<float>(x[i].e[k]));
             asm volatile("" : "+v"(lane));
             m = lanes_max<LW>(m);
-            const Exponent ex = exponent_of(m);
+            const float base = base_of(m);
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 if (lane + i * L < n_chunks) {
                     forget(x[i]);
-                    chunk_sums<T>(x[i], ex, s, t);
+                    chunk_sums<T>(x[i], base, s, t);
                     __builtin_amdgcn_sched_barrier(0);
                 }
         } else {
@@ -658,7 +653,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
                     rebase(m, mc, s, t);
                     m = mc;
                 }
-                chunk_sums<T>(y, exponent_of(m), s, t);
+                chunk_sums<T>(y, base_of(m), s, t);
             }
             const float mw = lanes_max<LW>(m);
             if (mw > m) rebase(m, mw, s, t);
@@ -686,9 +681,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
             parity ^= 1;                                   // the next row's exchange does not overwrite one that is still read
         }
         if (lane == 0) sums.s[5] += in.weight;
-        const Exponent ex = exponent_of(m);
+        const float base = base_of(m);
         const bool possible = za != neg_inf() && !(m == neg_inf() && s == 0.0f);          // logits that are all NaN leave m at -inf and s NaN
-        const RowGrad g = row_terms(a, in, inv_w, go, possible, fmaf(za, ex.scale, ex.shift), s, t, lane == 0, sums);
+        const RowGrad g = row_terms(a, in, inv_w, go, possible, exponent_of(za, base), s, t, lane == 0, sums);
         if (GRAD) {
             const bool nan = s != s;
             asm volatile("" : "+v"(lane));
@@ -698,7 +693,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
                     const int c = lane + i * L;
                     if (c < n_chunks) {
                         forget(x[i]);
-                        Chunk<T> y = grad_chunk<T>(x[i], c, action, ex, g, nan);
+                        Chunk<T> y = grad_chunk<T>(x[i], c, action, base, g, nan);
                         if (g.none) y.raw = u32x4{0, 0, 0, 0};
                         store_grad<T>(a, grad_ptr, i * L, lane, y);
                         __builtin_amdgcn_sched_barrier(0);
@@ -706,7 +701,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
                 }
             } else {
                 for (int c = lane; c < n_chunks; c += L) {
-                    Chunk<T> y = grad_chunk<T>(load_chunk<T>(a, row_ptr, row, c), c, action, ex, g, nan);
+                    Chunk<T> y = grad_chunk<T>(load_chunk<T>(a, row_ptr, row, c), c, action, base, g, nan);
                     if (g.none) y.raw = u32x4{0, 0, 0, 0};
                     store_grad<T>(a, grad_ptr, 0, c, y);
                 }

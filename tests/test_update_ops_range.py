@@ -1,0 +1,105 @@
+"""The update-side operators at the edges of their inputs' range: logits far from 0, policies next to their reference, values that are not
+numbers, calls that are refused.  Definitions in float64 as in test_update_ops.py, whose tolerance (ROW, derived there) is used per element:
+
+A logit's gradient is c1 ([j taken] - p_j) + ce p_j (log p_j + H) times the row's share of the weight.  p_j carries a relative error of at
+most 2^-24 (3 |log p_j| + 2) from its exponential and 7e-6 from the sum, log p_j + H an absolute one of 2^-22 (|log p_j| + H), c1 that of the
+row's terms: together less than ROW (1 + |log p_j|) p_j of the row's terms, and ROW of them where j is taken.  Below 1e-37 f32 leaves its
+normal range.  Where an action is not possible the gradient is 0 and nothing else.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_update_ops import DTYPES, ROW, check_policy, f64, half_step, oracle_policy, policy_inputs
+
+
+def masked_log_softmax(s):
+    z = torch.from_numpy(f64(s["logits"]))
+    if s["avail"] is not None:
+        z = torch.where(s["avail"].cpu() != 0, z, -math.inf)
+    return torch.log_softmax(z, 1).numpy()
+
+
+def gradient_excess(s, grad, scale, clip=0.2, entropy_coef=0.01, kl_coef=0.05):
+    """-> [rows, actions]: by how much the error of each element is above its bound (positive: wrong)"""
+    _, _, want, size = oracle_policy(s, clip=clip, entropy_coef=entropy_coef, kl_coef=kl_coef)
+    want = want * scale
+    logp = masked_log_softmax(s)
+    impossible = ~(logp > -np.inf)                         # and rows that nothing is possible in (NaN)
+    logp = np.where(impossible, 0.0, logp)
+    share = np.where(impossible, 0.0, np.exp(logp) * (1 + np.abs(logp)))
+    a = f64(s["actions"]).reshape(-1)
+    for r in np.flatnonzero((a >= 0) & (a < want.shape[1])):
+        share[r, int(a[r])] += 1.0
+    bound = ROW * scale * size[:, None] * share + half_step(want, s["logits"].dtype) + 1e-37 * scale * size[:, None]
+    return np.abs(grad - want) - np.where(impossible, 0.0, bound)
+
+
+def check_gradient(s, grad, scale, **kw):
+    excess = gradient_excess(s, f64(grad), scale, **kw)
+    assert np.all(excess <= 0), (float(np.nanmax(excess)), np.argwhere(~(excess <= 0))[:5])
+
+
+def around_the_logits(s, seed):
+    """old and reference log-probabilities near those of the logits as they are stored, away from the clip's borders"""
+    g = torch.Generator().manual_seed(seed)
+    rows = len(s["actions"])
+    lp = torch.from_numpy(masked_log_softmax(s))[torch.arange(rows), s["actions"].cpu()]
+    change = torch.randn(rows, generator=g, dtype=torch.float64) * 0.2
+    for border in (math.log(0.8), math.log(1.2)):
+        change = torch.where((change - border).abs() < 1e-3, torch.full_like(change, 0.01), change)
+    s["old"] = (lp - change).float().to(s["logits"].device)
+    s["ref"] = (lp + 0.2 * torch.randn(rows, generator=g, dtype=torch.float64)).float().to(s["logits"].device)
+    return lp
+
+
+def fused_autograd_and_value(s, scale=1.0, **coefs):
+    """The operator's three ways, checked against the definition."""
+    from diverse_conventions_amd import policy_loss, policy_loss_grad
+    kw = dict(kl_coef=0.05, ref_log_probs=s["ref"], active_masks=s["weights"], available_actions=s["avail"]) | coefs
+    fused = policy_loss_grad(s["logits"], s["actions"], s["old"], s["adv"], grad_scale=scale, **kw)
+    leaf = s["logits"].clone().requires_grad_()
+    loss, stats = policy_loss(leaf, s["actions"], s["old"], s["adv"], **kw)
+    (grad,) = torch.autograd.grad(loss, leaf, torch.tensor(scale, device="cuda"))
+    with torch.no_grad():
+        value = policy_loss(leaf, s["actions"], s["old"], s["adv"], **kw)
+    return fused, (loss.detach(), stats, grad), value
+
+
+# ------------------------------------------------------------------------------------------------- logits far from 0, finite masks
+RANGES = [("all", f) for f in (1e9, -1e9, 1e10, -1e10, -1e20, 1e30, -1e30, -6e4)] + [("few", f) for f in (-1e9, -1e10, -1e30, -6e4)] + \
+         [("shift", f) for f in (30.0, -30.0, 1e3, 1e4, 1e6)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [6, 13, 40, 300, 5000, 40000, 140000])
+@pytest.mark.parametrize("kind,value", RANGES, ids=lambda v: v if isinstance(v, str) else f"{v:g}")
+def test_policy_loss_of_logits_far_from_zero(kind, value, n, dtype):
+    """Rows of one large value (uniform), a few ordinary logits among a finite fill (whole wavefronts and lanes see only the fill), all
+    logits shifted: the loss is that of the differences, whatever they are relative to."""
+    dt = DTYPES[dtype]
+    if abs(value) > torch.finfo(dt).max:
+        pytest.skip("not a value of the type")
+    rows, scale = 3, 1024.0 if dtype == "f16" else 1.0
+    s = policy_inputs(n + 1, rows, n, torch.float32, "none", False, True, "cuda")
+    z = s["logits"]
+    if kind == "all":
+        z.fill_(value)
+    elif kind == "shift":
+        z += value
+    else:
+        keep = torch.tensor(sorted({1, n // 3, n // 2, n - 2}), device="cuda")
+        few = torch.full_like(z, value)
+        few[:, keep] = z[:, keep]
+        z.copy_(few)
+        s["actions"] = keep[torch.arange(rows, device="cuda") % len(keep)]
+    s["logits"] = z.to(dt)
+    around_the_logits(s, n)
+    fused, auto, plain = fused_autograd_and_value(s, scale)
+    for r in (fused, auto):
+        check_policy(s, r, scale)
+        check_gradient(s, r[2], scale)
+    assert torch.equal(plain[0], auto[0]) and torch.equal(plain[1], auto[1])
