@@ -249,8 +249,17 @@ __device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, const RowI
     float slope = cut ? 0.0f : -s1;
     float kl = 0.0f;
     if (a.ref_logp) {
-        const float d = in.ref_logp - lp, e = exp_fast(d) - 1.0f;
-        kl = e - d;
+        const float d = in.ref_logp - lp;
+        float e;                                           // exp(d) - 1
+        if (fabsf(d) < 0.25f) {
+            // next to the reference policy exp(d) - 1 - d is about d^2 / 2, and subtracting would leave its rounding, 2^-24, of either sign: the
+            // power series, cut where the next term is 2^-26 of the sum
+            kl = d * d * fmaf(d, fmaf(d, fmaf(d, fmaf(d, fmaf(d, 1.0f / 5040, 1.0f / 720), 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f);
+            e = d + kl;
+        } else {
+            e = exp_fast(d) - 1.0f;
+            kl = e - d;
+        }
         if (a.kl_coef != 0.0f) slope = slope - a.kl_coef * e;
     }
     if (leader) {

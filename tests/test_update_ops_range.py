@@ -103,3 +103,31 @@ def test_policy_loss_of_logits_far_from_zero(kind, value, n, dtype):
         check_policy(s, r, scale)
         check_gradient(s, r[2], scale)
     assert torch.equal(plain[0], auto[0]) and torch.equal(plain[1], auto[1])
+
+
+# ------------------------------------------------------------------------------------------------ policies next to their reference
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,rows", [(6, 4000), (13, 1000), (40, 1000), (5000, 200)])
+@pytest.mark.parametrize("spread", [0.0, 1e-4, 1e-3, 3e-2, 0.3, 2.0])
+def test_policy_loss_kl_next_to_the_reference_policy(spread, n, rows):
+    """kl = exp(d) - d - 1 with d = ref - lp is about d^2 / 2 and never negative.  lp carries at most
+    t = 2^-24 (3 (log n + 1) + 2 + min(n, 64) + 4 |lp| + 4): the sum's error (as above, with at most 64 roundings of a partial sum), the
+    logarithm's and the two products'; kl therefore |exp(d) - 1| t + exp(d) t^2, the rounding of a few operations (2^-21 of it) and, where
+    d is large enough to subtract, that of exp(d)."""
+    s = policy_inputs(n, rows, n, available="none", weights=False, device="cuda")
+    lp = around_the_logits(s, n).numpy()
+    g = torch.Generator().manual_seed(rows)
+    s["ref"] = torch.from_numpy(lp + spread * torch.randn(rows, generator=g, dtype=torch.float64).numpy()).float().cuda()
+    s["adv"].zero_()
+    fused, auto, _ = fused_autograd_and_value(s, kl_coef=1.0, entropy_coef=0.0)
+    d = f64(s["ref"]) - lp
+    kl = np.where(np.abs(d) < 1e-3, d * d / 2 * (1 + d / 3 + d * d / 12), np.expm1(d) - d)
+    t = 2.0 ** -24 * (3 * (math.log(n) + 1) + 6 + min(n, 64) + 4 * np.abs(lp))
+    bound = np.abs(np.expm1(d)) * t + np.exp(d) * t * t + 2.0 ** -21 * kl + np.where(np.abs(d) > 0.2, 2.0 ** -22 * (np.exp(d) + np.abs(d)), 0.0)
+    taken = np.arange(rows), f64(s["actions"]).astype(int)
+    want = -np.expm1(d) * -np.expm1(lp) / rows             # (1 - exp(d)) (1 - p) of the taken action
+    for loss, stats, grad in (fused, auto):
+        got = float(stats[2].double())
+        assert got >= 0 and abs(got - kl.mean()) <= bound.mean() + 2.0 ** -23 * kl.mean(), (got, kl.mean(), bound.mean())
+        assert abs(float(loss.double()) - kl.mean()) <= bound.mean() + 2.0 ** -23 * kl.mean()
+        assert np.all(np.abs(f64(grad)[taken] - want) <= (np.exp(d) * t + 4 * t * np.abs(np.expm1(d))) / rows)
