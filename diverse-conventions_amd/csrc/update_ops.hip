@@ -515,7 +515,7 @@ __device__ __forceinline__ void store_grad(const PolicyLossArgs &a, T *row_ptr, 
     }
 }
 
-// `nan`: the row's sums are not numbers, and 0 times them is not what a masked place gets
+// `nan`: the row's sums or coefficients are not finite, and 0 times them is not what a masked place gets
 template <typename T>
 __device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &x, int c, int action, float base, const RowGrad &g, bool nan) {
     constexpr int V = Chunk<T>::V;
@@ -694,7 +694,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) __attribute__((amdgpu_waves_per_
         const bool possible = za != neg_inf() && !(m == neg_inf() && s == 0.0f);          // logits that are all NaN leave m at -inf and s NaN
         const RowGrad g = row_terms(a, in, inv_w, go, possible, exponent_of(za, base), s, t, lane == 0, sums);
         if (GRAD) {
-            const bool nan = s != s;
+            const bool nan = !(s + fabsf(g.c1) + fabsf(g.a1) + fabsf(g.a0) < __builtin_inff());
             asm volatile("" : "+v"(lane));
             if (C) {
 #pragma unroll

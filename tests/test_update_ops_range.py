@@ -131,3 +131,30 @@ def test_policy_loss_kl_next_to_the_reference_policy(spread, n, rows):
         assert got >= 0 and abs(got - kl.mean()) <= bound.mean() + 2.0 ** -23 * kl.mean(), (got, kl.mean(), bound.mean())
         assert abs(float(loss.double()) - kl.mean()) <= bound.mean() + 2.0 ** -23 * kl.mean()
         assert np.all(np.abs(f64(grad)[taken] - want) <= (np.exp(d) * t + 4 * t * np.abs(np.expm1(d))) / rows)
+
+
+# ----------------------------------------------------------------------------------------------------- what is not a number beside masks
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [6, 40, 300, 5000, 70001, 140000])
+def test_policy_loss_impossible_actions_get_zero_in_every_row(n, dtype):
+    """Rows whose terms are not finite though their logits are: an advantage or a log-probability that is NaN, a ratio or a KL term that
+    overflows.  Their impossible actions still get 0, the other rows are as ever."""
+    s = policy_inputs(n, 7, n, DTYPES[dtype], "rows", False, True, "cuda")
+    lp = around_the_logits(s, n)
+    clean = s["logits"].clone()
+    free = torch.where(torch.arange(n) == (s["actions"][6].item() + 1) % n, -math.inf, 0.0)      # -inf as a mask of its own
+    s["logits"][6] = clean[6] + free.to(clean)
+    s["adv"][1] = math.nan
+    s["old"][2], s["adv"][2] = float(lp[2]) - 200.0, -1.0                   # ratio exp(200)
+    s["old"][3] = math.nan
+    s["ref"][4] = math.nan
+    s["ref"][5] = 300.0
+    s["ref"][6] = 300.0
+    impossible = (s["avail"] == 0) | (s["logits"] == -math.inf)
+    assert impossible.any()
+    fused, auto, _ = fused_autograd_and_value(s)
+    for _, _, grad in (fused, auto):
+        assert not grad[impossible].isnan().any() and not grad[impossible].any()
+        assert torch.isfinite(grad[0]).all()
+        assert all(not torch.isfinite(grad[r]).all() for r in range(1, 7))
