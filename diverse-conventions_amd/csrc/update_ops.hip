@@ -33,7 +33,7 @@ template <typename T> struct Chunk {                       // 16 bytes of elemen
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -1e30f;                          // floor of log-probabilities in products with a probability of 0
+constexpr float kLowest = -1e4f;                           // floor of exponents in products with 2^v, which is 0 long before
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 // The hardware's own exp2, log2 and reciprocal: 1 ulp, where arguments below the normal range do not matter (a probability of 2^-127
 // counts as 0 next to one of 1).  The library functions around them cost more than the memory traffic of a short row.

@@ -158,3 +158,18 @@ def test_policy_loss_impossible_actions_get_zero_in_every_row(n, dtype):
         assert not grad[impossible].isnan().any() and not grad[impossible].any()
         assert torch.isfinite(grad[0]).all()
         assert all(not torch.isfinite(grad[r]).all() for r in range(1, 7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 13, 40, 5000, 70001])
+def test_policy_loss_gradient_of_a_large_scale(n):
+    """A gradient scaled by 1e12: actions whose probability is 0 in f32 get 0, masked ones too."""
+    s = policy_inputs(n, 5, n, available="rows", weights=False, device="cuda")
+    a = s["actions"]
+    far = (torch.rand((5, n), device="cuda", generator=torch.Generator("cuda").manual_seed(n)) < 0.5) & (torch.arange(n, device="cuda") != a[:, None])
+    s["logits"][far] = -1e30
+    s["logits"][0, (a[0] + 1) % n] = -1e30
+    around_the_logits(s, n)
+    fused, auto, _ = fused_autograd_and_value(s, 1e12)
+    for r in (fused, auto):
+        check_gradient(s, r[2], 1e12)
