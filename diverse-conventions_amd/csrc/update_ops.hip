@@ -34,6 +34,7 @@ template <typename T> struct Chunk {                       // 16 bytes of elemen
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e4f;                           // floor of exponents in products with 2^v, which is 0 long before
+constexpr float kLargest = 3.4028235e38f;
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 // The hardware's own exp2, log2 and reciprocal: 1 ulp, where arguments below the normal range do not matter (a probability of 2^-127
 // counts as 0 next to one of 1).  The library functions around them cost more than the memory traffic of a short row.
@@ -238,7 +239,8 @@ __device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, const RowI
     RowGrad g = {0.0f, 0.0f, 0.0f, true};
     if (!possible) return g;
     const float log_s = log2_fast(s), inv_s = rcp_fast(s);
-    const float lp = (va - log_s) * kLn2;
+    // an action beyond the range of exponents has the lowest log-probability, not -inf: exp(d) - d below is inf, not inf - inf
+    const float lp_any = (va - log_s) * kLn2, lp = lp_any < -kLargest ? -kLargest : lp_any;
     const float entropy = (log_s - t * inv_s) * kLn2;
     const float adv = in.adv, weight = in.weight;
     const float ratio = exp_fast(lp - in.old_logp);

@@ -173,3 +173,21 @@ def test_policy_loss_gradient_of_a_large_scale(n):
     fused, auto, _ = fused_autograd_and_value(s, 1e12)
     for r in (fused, auto):
         check_gradient(s, r[2], 1e12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 40, 5000, 70001])
+def test_policy_loss_kl_of_an_action_of_no_probability_is_infinite(n):
+    """The taken action at the type's lowest value: its log-probability is beyond f32 in units of log 2, exp(ref - lp) - (ref - lp) - 1 is
+    infinite and not NaN; without the KL term the row is an ordinary one of ratio 0."""
+    for value in (torch.finfo(torch.float32).min, -3e38):
+        s = policy_inputs(n, 4, n, available="none", weights=False, device="cuda")
+        s["logits"][1, s["actions"][1]] = value
+        fused, auto, plain = fused_autograd_and_value(s)
+        for loss, stats, *_ in (fused, auto, plain):
+            assert float(loss) == math.inf and float(stats[2]) == math.inf and torch.isfinite(stats[[0, 1, 3, 4]]).all()
+        s["ref"] = None
+        fused, auto, plain = fused_autograd_and_value(s)
+        for r in (fused, auto):
+            check_policy(s, r)
+            check_gradient(s, r[2], 1.0)
