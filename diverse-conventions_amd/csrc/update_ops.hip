@@ -245,7 +245,8 @@ __device__ __forceinline__ RowGrad row_terms(const PolicyLossArgs &a, const RowI
     const float adv = in.adv, weight = in.weight;
     const float ratio = exp_fast(lp - in.old_logp);
     const float kept = fminf(fmaxf(ratio, a.clip_lo), a.clip_hi);
-    const float s1 = ratio * adv, s2 = kept * adv;
+    const auto times_adv = [&](float x) { return adv == 0.0f && x == __builtin_inff() ? 0.0f : x * adv; };        // a ratio beyond f32 is a number
+    const float s1 = times_adv(ratio), s2 = times_adv(kept);
     const float policy = -(s1 != s1 || s2 != s2 ? s1 + s2 : fminf(s1, s2));
     const bool cut = (adv > 0.0f && ratio > a.clip_hi) || (adv < 0.0f && ratio < a.clip_lo);
     float slope = cut ? 0.0f : -s1;

@@ -191,3 +191,26 @@ def test_policy_loss_kl_of_an_action_of_no_probability_is_infinite(n):
         for r in (fused, auto):
             check_policy(s, r)
             check_gradient(s, r[2], 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 40, 5000])
+def test_policy_loss_of_a_zero_advantage_and_a_ratio_beyond_f32(n):
+    """An advantage of 0 contributes 0 however large the ratio: old log-probabilities 100 below, with and without a clip."""
+    s = policy_inputs(n, 4, n, available="none", weights=False, ref=False, device="cuda")
+    lp = around_the_logits(s, n)
+    s["old"][1], s["adv"][1], s["ref"] = float(lp[1]) - 100.0, 0.0, None
+    s["old"][2], s["adv"][2] = float(lp[2]) - 100.0, 1.5                    # clipped: no gradient through the ratio
+    for clip in (0.2, math.inf):
+        if clip == math.inf:
+            s["adv"][2] = 0.0
+        fused, auto, plain = fused_autograd_and_value(s, clip_param=clip)
+        want, means, _, size = oracle_policy(s, clip=clip, kl_coef=0.05)
+        size[1:3] = 1.0                                    # the ratio's size times 0 is no measure; the terms are below 1
+        for r in (fused, auto, plain):
+            assert abs(float(r[0]) - want) <= ROW * (abs(want) + size.sum()), (float(r[0]), want)
+            assert abs(float(r[1][0]) - means[0]) <= ROW * (abs(means[0]) + size.sum()) and float(r[1][4]) == math.inf
+        for r in (fused, auto):
+            check_gradient(s, r[2], 1.0, clip=clip)
+            entropy_only = f64(r[2])[1:3]
+            assert np.all(np.abs(entropy_only) <= 0.01 * (1 + math.log(n)))
