@@ -873,11 +873,12 @@ __device__ __forceinline__ float value_sample(const ValueLossArgs &a, float v, f
         slope = e0;
     }
     float worst = h0;
-    if (a.clip >= 0.0f && fabsf(step) > a.clip) {
+    if (a.clip >= 0.0f && !(fabsf(step) <= a.clip)) {       // also where v0 is not a number: neither is e1 then
         const float e1 = y - (v0 + copysignf(a.clip, step));
         h1 = a.delta >= 0.0f && fabsf(e1) > a.delta ? a.delta * (fabsf(e1) - 0.5f * a.delta) : 0.5f * e1 * e1;
         free_ = !(h0 < h1);
         worst = free_ ? h0 : h1;
+        if (h1 != h1) worst = slope = h1;
     }
     sum += static_cast<double>(w) * static_cast<double>(worst);
     return free_ ? -scale * w * slope : 0.0f;

@@ -107,7 +107,8 @@ int oc_policy_loss(const oc_policy_loss_args *args, int what, void *d_workspace,
 /* Clipped value loss and its gradient (R_MAPPO.cal_value_loss, train/MAPPO/r_mappo.py; huber_loss / mse_loss of train/MAPPO/utils/util.py):
  *   y = (return - mean) / std;  e0 = y - v;  e1 = y - (v0 + clamp(v - v0, -c, c));  loss = sum w max(h(e0), h(e1)) / sum w
  * with h Huber's of huber_delta (< 0: e^2 / 2); clip_param < 0: h(e0) alone; std must be positive.  The gradient is that of h(e0) where |v - v0| <= c or
- * h(e0) >= h(e1), else 0.  Samples of weight 0 are left out whatever they hold; no weight at all gives a loss of 0.
+ * h(e0) >= h(e1), else 0; where one of them is NaN the loss and the sample's gradient are.  Samples of weight 0 are left out whatever they
+ * hold; no weight at all gives a loss of 0.
  * Passes, d_loss, d_weight (the sum of w), grad_scale and workspace as oc_policy_loss. */
 typedef struct {
     const void *d_values;

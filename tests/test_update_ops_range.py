@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_update_ops import DTYPES, ROW, check_policy, f64, half_step, oracle_policy, policy_inputs
+from test_update_ops import DTYPES, ROW, check_policy, f64, half_step, oracle_policy, policy_inputs, value_inputs
 
 
 def masked_log_softmax(s):
@@ -214,3 +214,23 @@ def test_policy_loss_of_a_zero_advantage_and_a_ratio_beyond_f32(n):
             check_gradient(s, r[2], 1.0, clip=clip)
             entropy_only = f64(r[2])[1:3]
             assert np.all(np.abs(entropy_only) <= 0.01 * (1 + math.log(n)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,at", [(40, 5), (41, 40), (5003, 5002), (70000, 333)])
+def test_value_loss_shows_old_values_that_are_not_numbers(n, at):
+    """max(h(e0), h(e1)) is not a number where the rollout's value is none; without the clipped branch that value is not looked at."""
+    from diverse_conventions_amd import value_loss, value_loss_grad
+    v, v0, ret, w = value_inputs(n, n, torch.float32, True, None)
+    v0[at], w[at] = math.nan, 1.0
+    others = torch.arange(n, device="cuda") != at
+    for delta in (10.0, None):
+        leaf = v.clone().requires_grad_()
+        one = value_loss(leaf, v0, ret, huber_delta=delta, active_masks=w)
+        for loss, grad in (value_loss_grad(v, v0, ret, huber_delta=delta, active_masks=w), (one, torch.autograd.grad(one, leaf)[0])):
+            assert torch.isnan(loss) and torch.isnan(grad[at]) and torch.isfinite(grad[others]).all()
+        loss, grad = value_loss_grad(v, v0, ret, clip_param=None, huber_delta=delta, active_masks=w)
+        assert torch.isfinite(loss) and torch.isfinite(grad).all()
+        skipped = torch.where(others, w, 0.0)
+        loss, grad = value_loss_grad(v, v0, ret, huber_delta=delta, active_masks=skipped)
+        assert torch.isfinite(loss) and torch.isfinite(grad).all()
