@@ -112,10 +112,11 @@ __device__ __forceinline__ double block_sums(const double (&x)[N], double (*part
     return sum;
 }
 
-// The taken action of a row, -1 when it is none of 0 .. n - 1 (also a float that is NaN or lies outside).
+// The taken action of a row, -1 when it is none of 0 .. n - 1 (also a float that is NaN or lies outside [0, n): the comparison with n is one
+// of whole numbers, 2^24 + 1 is no float).
 __device__ __forceinline__ int checked_action(int v, int n) { return v >= 0 && v < n ? v : -1; }
 __device__ __forceinline__ int checked_action(long long v, int n) { return v >= 0 && v < n ? static_cast<int>(v) : -1; }
-__device__ __forceinline__ int checked_action(float f, int n) { return f > -1.0f && f < static_cast<float>(n) ? static_cast<int>(f) : -1; }
+__device__ __forceinline__ int checked_action(float f, int n) { return f >= 0.0f && f < 0x1p30f ? checked_action(static_cast<int>(f), n) : -1; }
 
 // `first`: a row that is the same for all lanes, `i`: this lane's behind it
 __device__ __forceinline__ int action_of(const PolicyLossArgs &a, long long first, uint32_t i = 0) {

@@ -17,7 +17,7 @@ def policy_loss(logits, actions, old, adv, clip=0.2, entropy_coef=0.01, kl_coef=
     grad, size, sums, total = np.zeros_like(z), np.zeros(rows), np.zeros(5), 0.0
     old, adv = (np.asarray(t, np.float64).reshape(-1) for t in (old, adv))
     ref = None if ref is None else np.asarray(ref, np.float64).reshape(-1)
-    valid = [r for r in range(rows) if -1 < a[r] < n]
+    valid = [r for r in range(rows) if 0 <= a[r] < n]
     total = sum(w[r] for r in valid)
     for r in valid:
         j = int(a[r])

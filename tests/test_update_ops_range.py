@@ -234,3 +234,38 @@ def test_value_loss_shows_old_values_that_are_not_numbers(n, at):
         skipped = torch.where(others, w, 0.0)
         loss, grad = value_loss_grad(v, v0, ret, huber_delta=delta, active_masks=skipped)
         assert torch.isfinite(loss) and torch.isfinite(grad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [6, 40, 5000])
+def test_policy_loss_actions_stored_as_floats(n):
+    """Outside [0, actions) is padding, also between -1 and 0; -0.0 is action 0."""
+    s = policy_inputs(n, 8, n, available="none", device="cuda")
+    s["weights"][:] = 1.0
+    s["actions"] = torch.tensor([-0.5, -0.0, n - 1.0, float(n), math.nan, math.inf, -1e-30, -1.0], device="cuda")
+    floats, _, _ = fused_autograd_and_value(s)
+    s["actions"] = torch.tensor([-1, 0, n - 1, n, -1, -1, -1, -1], device="cuda")
+    whole, _, _ = fused_autograd_and_value(s)
+    assert all(torch.equal(a, b) for a, b in zip(floats, whole))
+    check_policy(s, floats)
+    # 1024 rows and more: the weights are added up by a launch of their own
+    big = policy_inputs(n, 1500 + n % 7, min(n, 40), available="none", weights=False, device="cuda")
+    a = torch.where(torch.arange(len(big["actions"]), device="cuda") % 3 == 0, -0.5, big["actions"].float())
+    big["actions"] = a
+    floats, _, _ = fused_autograd_and_value(big)
+    big["actions"] = torch.where(a < 0, -1, a.long())
+    whole, _, _ = fused_autograd_and_value(big)
+    assert all(torch.equal(x, y) for x, y in zip(floats, whole))
+
+
+@pytest.mark.gpu
+def test_policy_loss_actions_stored_as_floats_beyond_their_whole_numbers():
+    """2^24 + 1 actions: the number of actions is no float of its own, its last action is."""
+    from diverse_conventions_amd import policy_loss_grad
+    n = 2 ** 24 + 1
+    z, one = torch.zeros((1, n), dtype=torch.bfloat16, device="cuda"), torch.ones(1, device="cuda")
+    last = torch.tensor([n - 1], device="cuda")
+    assert int(last.float()) == n - 1
+    want = policy_loss_grad(z, last, -math.log(n) * one, one)
+    got = policy_loss_grad(z, last.float(), -math.log(n) * one, one)
+    assert float(want[1][4]) > 0.9 and all(torch.equal(a, b) for a, b in zip(got, want))
