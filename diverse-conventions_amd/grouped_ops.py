@@ -8,6 +8,7 @@ from torch.autograd.function import once_differentiable
 
 from . import native
 from .engine import _raw_stream
+from .update_ops import _refuse_tangents
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -85,6 +86,7 @@ def grouped_linear(x, weight, offsets, bias=None):
     depend on timing.  -> y [rows, out_features]
 
     The segments of `pairing_segments` are such groups: the critics of all pairings (`segment_critics`) learn in one pass."""
+    _refuse_tangents("grouped_linear", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GroupedLinear.apply(x, weight, offsets, bias)
     return _forward(x, weight, offsets, bias)

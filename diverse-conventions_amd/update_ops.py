@@ -9,6 +9,7 @@ import math
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import native
@@ -34,6 +35,12 @@ def _workspace(size_of, device):
     if size is None:
         size = _workspace_bytes[size_of] = getattr(native.lib(), size_of)()
     return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _refuse_tangents(what, *tensors):
+    """These operators have no forward-mode derivative; read by address, a dual tensor would lose its tangent without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} does not support forward mode automatic differentiation")
 
 
 def _rows_f32(name, t, n, device):
@@ -137,6 +144,7 @@ def policy_loss(logits, actions, old_log_probs, advantages, clip_param=0.2, entr
 
     `loss.backward()` recomputes the softmax from the logits: no [rows, actions] tensor is kept.  `policy_loss_grad` gives the gradient at once.
     """
+    _refuse_tangents("policy_loss", logits, old_log_probs, advantages, ref_log_probs, active_masks)
     if logits.requires_grad and torch.is_grad_enabled():
         return _PolicyLoss.apply(logits, actions, old_log_probs, advantages, ref_log_probs, active_masks, available_actions, clip_param, entropy_coef, kl_coef)
     return _PolicyCall(logits, actions, old_log_probs, advantages, clip_param, entropy_coef, kl_coef, ref_log_probs, active_masks,
@@ -148,6 +156,7 @@ def policy_loss_grad(logits, actions, old_log_probs, advantages, clip_param=0.2,
     """`policy_loss` and its gradient in one pass over the logits, outside autograd: -> (loss, stats, grad), grad = grad_scale * d loss /
     d logits, contiguous, of the logits' shape and type, for `logits.backward(grad)`.  grad_scale: loss scaling for float16, whose range a
     mean over many rows leaves."""
+    _refuse_tangents("policy_loss_grad", logits, old_log_probs, advantages, ref_log_probs, active_masks)
     return _PolicyCall(logits, actions, old_log_probs, advantages, clip_param, entropy_coef, kl_coef, ref_log_probs, active_masks,
                        available_actions).forward(True, grad_scale)
 
@@ -227,6 +236,7 @@ def value_loss(values, value_preds, returns, clip_param=0.2, huber_delta=10.0, a
     values f32 / bf16 / f16, value_preds (v0: the values of the rollout), returns and active_masks (None: 1) f32, all contiguous with as
     many elements; h: Huber's loss of `huber_delta`, None: e^2 / 2; clip_param None: without the clipped branch; value_normalizer: None, a
     (mean, std) pair or an object with `running_mean_var()`, as in `gae_returns`.  Samples of weight 0 may hold anything.  -> f32 scalar."""
+    _refuse_tangents("value_loss", values, value_preds, returns, active_masks)
     norm = _normalizer(value_normalizer)
     if values.requires_grad and torch.is_grad_enabled():
         return _ValueLoss.apply(values, value_preds, returns, active_masks, clip_param, huber_delta, norm)
@@ -235,6 +245,7 @@ def value_loss(values, value_preds, returns, clip_param=0.2, huber_delta=10.0, a
 
 def value_loss_grad(values, value_preds, returns, clip_param=0.2, huber_delta=10.0, active_masks=None, value_normalizer=None, grad_scale=1.0):
     """`value_loss` and its gradient in one pass, outside autograd: -> (loss, grad_scale * d loss / d values of the values' shape and type)."""
+    _refuse_tangents("value_loss_grad", values, value_preds, returns, active_masks)
     return _ValueCall(values, value_preds, returns, clip_param, huber_delta, active_masks, _normalizer(value_normalizer)).forward(True, grad_scale)
 
 
@@ -276,6 +287,7 @@ def clip_grad_norm(grads, max_norm=None, norm_type=2.0, out=None):
     plain = torch.Tensor                                 # hundreds of tensors: one cheap look at each property, all at once
     tensors = [g if type(g) is plain else g.grad if isinstance(g, torch.nn.Parameter) else g for g in grads]
     tensors = [t for t in tensors if t is not None]
+    _refuse_tangents("clip_grad_norm", *tensors)
     if norm_type not in (2, 2.0, math.inf, "inf"):
         raise ValueError("norm_type must be 2 or inf")
     if max_norm is not None and not max_norm >= 0:
