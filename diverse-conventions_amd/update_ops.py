@@ -2,7 +2,7 @@
 Thin torch front-ends of the C ABI (include/overcooked_ops.h), next to `gae_returns` / `normalize_advantages` / `MinibatchSource`.
 
 Every call works on its arguments' GPU and on that device's current stream, allocates its results and workspace from torch's caching
-allocator, keeps nothing between calls and never synchronises with the host.
+allocator and keeps nothing between calls.  Nothing synchronises with the host but a value normaliser given as an object, which is read back.
 """
 import ctypes
 import math
@@ -235,7 +235,9 @@ def value_loss(values, value_preds, returns, clip_param=0.2, huber_delta=10.0, a
 
     values f32 / bf16 / f16, value_preds (v0: the values of the rollout), returns and active_masks (None: 1) f32, all contiguous with as
     many elements; h: Huber's loss of `huber_delta`, None: e^2 / 2; clip_param None: without the clipped branch; value_normalizer: None, a
-    (mean, std) pair or an object with `running_mean_var()`, as in `gae_returns`.  Samples of weight 0 may hold anything.  -> f32 scalar."""
+    (mean, std) pair or an object with `running_mean_var()`, as in `gae_returns` -- the object is read back to the host at the call: it waits
+    for the GPU, and a captured graph wants the pair, which stays what it was at the capture.  Samples of weight 0 may hold anything.
+    -> f32 scalar."""
     _refuse_tangents("value_loss", values, value_preds, returns, active_masks)
     norm = _normalizer(value_normalizer)
     if values.requires_grad and torch.is_grad_enabled():

@@ -296,3 +296,21 @@ def test_forward_mode_is_refused(device):
                 call()
         if device == "cuda":
             policy_loss(z, a, r, r), value_loss(r, r, r), grouped_linear(x, w, o, b), clip_grad_norm([x], 1.0)
+
+
+@pytest.mark.gpu
+def test_value_loss_with_a_normalizer_object():
+    """An object with running_mean_var() is read back at the call and gives what its (mean, standard deviation) pair gives."""
+    from diverse_conventions_amd import value_loss, value_loss_grad
+
+    class Normalizer:
+        def running_mean_var(self):
+            return torch.tensor([1.5], device="cuda"), torch.tensor([6.25], device="cuda")
+
+    v, v0, ret, w = value_inputs(3, 5000, torch.float32, True, (1.5, 2.5))
+    for a, b in zip(value_loss_grad(v, v0, ret, active_masks=w, value_normalizer=Normalizer()), value_loss_grad(v, v0, ret, active_masks=w, value_normalizer=(1.5, 2.5))):
+        assert torch.equal(a, b)
+    leaf = v.clone().requires_grad_()
+    (x,) = torch.autograd.grad(value_loss(leaf, v0, ret, active_masks=w, value_normalizer=Normalizer()), leaf)
+    (y,) = torch.autograd.grad(value_loss(leaf, v0, ret, active_masks=w, value_normalizer=(1.5, 2.5)), leaf)
+    assert torch.equal(x, y)
