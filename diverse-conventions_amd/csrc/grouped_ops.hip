@@ -756,8 +756,30 @@ int check_grouped(const oc_grouped_linear_args *p, const char *who) {
     return OC_OK;
 }
 
+// What a backward pass computes and where its f32 parts lie in the workspace: dx's, then dW's, then db's, each only where that gradient is
+// asked for and its sums are cut.  The workspace's size and its use both come from here.
+struct BackwardPlan {
+    RowsPlan rows;
+    WeightPlan weights;
+    long long n_w, n_b;                                    // elements to be joined, 0: written at once
+    long long at_w, at_b, floats;                          // dW's parts, db's parts, the end
+};
+
+BackwardPlan backward_plan(const oc_grouped_linear_args *p, bool dx, bool dw, bool db) {
+    const int K = p->in_features, N = p->out_features;
+    BackwardPlan b;
+    b.rows = rows_plan(p->type, p->rows, p->groups, K, N);
+    b.weights = weight_plan(p->type, p->rows, p->groups, K, N);
+    b.n_w = dw && b.weights.splits > 1 ? static_cast<long long>(p->groups) * N * K : 0;
+    b.n_b = db && b.weights.bias_splits > 1 ? static_cast<long long>(p->groups) * N : 0;
+    b.at_w = dx ? rows_parts(b.rows, p->rows, K) : 0;
+    b.at_b = b.at_w + b.n_w * b.weights.splits;
+    b.floats = b.at_b + b.n_b * b.weights.bias_splits;
+    return b;
+}
+
 template <typename T>
-hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &base, float *parts, hipStream_t s) {
+hipError_t backward_type(const oc_grouped_linear_args *p, const BackwardPlan &plan, const GroupedArgs &base, float *parts, hipStream_t s) {
     hipError_t e = hipSuccess;
     const int K = p->in_features, N = p->out_features, V = p->type == OC_F32 ? 4 : 8;
     if (p->d_dx && p->rows > 0) {
@@ -765,24 +787,19 @@ hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &bas
         a.I = p->d_weight; a.J = p->d_dy; a.out = p->d_dx;
         a.ld_i = K; a.ld_j = N; a.ld_out = K;
         a.ni = K; a.red = N;
-        const RowsPlan plan = rows_plan(p->type, p->rows, p->groups, K, N);
-        e = launch_rows<T, true, false>(a, plan, parts, aligned_rows(p->d_weight, K, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
+        e = launch_rows<T, true, false>(a, plan.rows, parts, aligned_rows(p->d_weight, K, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
         if (e != hipSuccess) return e;
-        parts += rows_parts(plan, p->rows, K);
     }
-    const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
     if (p->d_dweight || p->d_dbias) {
         GroupedArgs a = base;
         a.I = p->d_x; a.J = p->d_dy;
         a.ld_i = p->x_stride; a.ld_j = N; a.ld_out = K;
-        a.ni = K; a.nj = N; a.splits = plan.splits; a.bias_splits = plan.bias_splits;
-        const long long n_w = p->d_dweight && plan.splits > 1 ? static_cast<long long>(p->groups) * N * K : 0;
-        const long long n_b = p->d_dbias && plan.bias_splits > 1 ? static_cast<long long>(p->groups) * N : 0;
-        float *const parts_b = parts + n_w * plan.splits;
-        a.out = n_w ? static_cast<void *>(parts) : p->d_dweight;
-        a.bias_out = n_b ? static_cast<void *>(parts_b) : p->d_dbias;
-        e = launch_weights<T>(a, plan, aligned_rows(p->d_x, p->x_stride, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
-        if (e == hipSuccess) e = launch_join<T>(parts, p->d_dweight, n_w, plan.splits, parts_b, p->d_dbias, n_b, plan.bias_splits, s);
+        a.ni = K; a.nj = N; a.splits = plan.weights.splits; a.bias_splits = plan.weights.bias_splits;
+        a.out = plan.n_w ? static_cast<void *>(parts + plan.at_w) : p->d_dweight;
+        a.bias_out = plan.n_b ? static_cast<void *>(parts + plan.at_b) : p->d_dbias;
+        e = launch_weights<T>(a, plan.weights, aligned_rows(p->d_x, p->x_stride, p->type) && aligned_rows(p->d_dy, N, p->type) && K % V == 0 && N % V == 0, s);
+        if (e == hipSuccess)
+            e = launch_join<T>(parts + plan.at_w, p->d_dweight, plan.n_w, plan.weights.splits, parts + plan.at_b, p->d_dbias, plan.n_b, plan.weights.bias_splits, s);
     }
     return e;
 }
@@ -791,15 +808,12 @@ hipError_t backward_type(const oc_grouped_linear_args *p, const GroupedArgs &bas
 
 extern "C" int64_t oc_grouped_linear_workspace_bytes(const oc_grouped_linear_args *p, int backward) {
     if (check_grouped(p, "oc_grouped_linear_workspace_bytes") != OC_OK) return -1;
-    const int K = p->in_features, N = p->out_features;
     long long floats;
     if (!backward) {
-        floats = rows_parts(rows_plan(p->type, p->rows, p->groups, N, K), p->rows, N);
+        floats = rows_parts(rows_plan(p->type, p->rows, p->groups, p->out_features, p->in_features), p->rows, p->out_features);
     } else {
-        const WeightPlan plan = weight_plan(p->type, p->rows, p->groups, K, N);
-        const long long out = static_cast<long long>(p->groups) * N;
-        floats = rows_parts(rows_plan(p->type, p->rows, p->groups, K, N), p->rows, K) + (plan.splits > 1 ? plan.splits * out * K : 0) +
-                 (plan.bias_splits > 1 ? plan.bias_splits * out : 0);
+        const bool any = p->d_dx || p->d_dweight || p->d_dbias;            // no output known yet: room for all of them
+        floats = backward_plan(p, p->d_dx || !any, p->d_dweight || !any, p->d_dbias || !any).floats;
     }
     return floats * static_cast<long long>(sizeof(float));
 }
@@ -831,15 +845,17 @@ extern "C" int oc_grouped_linear(const oc_grouped_linear_args *p, void *d_worksp
 extern "C" int oc_grouped_linear_backward(const oc_grouped_linear_args *p, void *d_workspace, void *stream) {
     if (const int rc = check_grouped(p, "oc_grouped_linear_backward")) return rc;
     if (p->rows > 0 && !p->d_dy) return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: d_dy is NULL");
-    const int64_t need = oc_grouped_linear_workspace_bytes(p, 1);
-    if (need > 0 && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
-        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: needs a workspace of %lld bytes", static_cast<long long>(need));
+    if (!p->d_dx && !p->d_dweight && !p->d_dbias) return OC_OK;
+    const BackwardPlan plan = backward_plan(p, p->d_dx, p->d_dweight, p->d_dbias);
+    if (plan.floats > 0 && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 4))
+        return oc_internal_fail(OC_ERR_INVALID_ARG, "oc_grouped_linear_backward: needs a workspace of %lld bytes", plan.floats * static_cast<long long>(sizeof(float)));
     GroupedArgs a = {};
     a.offsets = p->d_offsets; a.rows = p->rows; a.groups = p->groups; a.offsets64 = p->offsets64 != 0; a.splits = 1;
     const OcDeviceScope on_device(oc_device_of_pointer(p->d_weight));
     hipStream_t s = static_cast<hipStream_t>(stream);
     float *parts = static_cast<float *>(d_workspace);
-    const hipError_t e = p->type == OC_F32 ? backward_type<float>(p, a, parts, s) : p->type == OC_BF16 ? backward_type<__bf16>(p, a, parts, s)
-                                                                                                       : backward_type<_Float16>(p, a, parts, s);
+    const hipError_t e = p->type == OC_F32    ? backward_type<float>(p, plan, a, parts, s)
+                         : p->type == OC_BF16 ? backward_type<__bf16>(p, plan, a, parts, s)
+                                              : backward_type<_Float16>(p, plan, a, parts, s);
     return e == hipSuccess ? OC_OK : oc_internal_fail(OC_ERR_HIP, "oc_grouped_linear_backward: %s", hipGetErrorString(e));
 }

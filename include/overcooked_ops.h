@@ -143,7 +143,8 @@ int oc_grad_norm_clip(int32_t n_tensors, const void *const *d_grads, void *const
  * Products run on the matrix cores with f32 accumulation; results are rounded once.  d_offsets [groups + 1] must not decrease; entries
  * are clamped into [0, rows], a group may be empty (its gradients are 0).  Sums over many rows (dweight, dbias) and products of few rows
  * over many features are cut into f32 parts, which the workspace holds (oc_grouped_linear_workspace_bytes of the pass; 0 if none is needed,
- * < 0 for wrong arguments) and which are added up in a fixed order. */
+ * < 0 for wrong arguments) and which are added up in a fixed order.  The size of a backward pass is that of the gradients whose pointers are
+ * set when it is asked for -- the same as in the call -- or of all three if none is set yet. */
 typedef struct {
     const void *d_x;                   /* [rows] of in_features values, x_stride elements apart */
     const void *d_weight;              /* [groups][out_features][in_features] */
