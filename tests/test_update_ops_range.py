@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_update_ops import DTYPES, ROW, check_policy, f64, half_step, oracle_policy, policy_inputs, value_inputs
+from test_update_ops import DTYPES, POLICY_SIZES, ROW, check_policy, f64, half_step, oracle_policy, policy_inputs, value_inputs
 
 
 def masked_log_softmax(s):
@@ -314,3 +314,61 @@ def test_value_loss_with_a_normalizer_object():
     (x,) = torch.autograd.grad(value_loss(leaf, v0, ret, active_masks=w, value_normalizer=Normalizer()), leaf)
     (y,) = torch.autograd.grad(value_loss(leaf, v0, ret, active_masks=w, value_normalizer=(1.5, 2.5)), leaf)
     assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------- every element of the gradient
+def gradient_case(rows, n, k, dtype, device):
+    """The inputs of the sizes' test in test_update_ops.py; float16 gradients are scaled so that those of long rows stay above its subnormals."""
+    available, weights, ref = [("none", False, False), ("rows", True, True), ("one", True, False)][k]
+    s = policy_inputs(rows * 7 + n + k, rows, n, DTYPES[dtype], available, weights, ref, device)
+    return s, 4096.0 if dtype == "f16" and n > 100 else 64.0 if dtype == "f16" else 1.0
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,n", [(400, 6), (40, 255), (5, 1000), (2, 16385), (1, 50021), (2, 70001), (1, 131072)])
+def test_the_gradient_check_notices_what_is_left_out(rows, n, dtype):
+    """On the definition itself: rounded to the type it passes; without the actions that were not taken, or without a row's last piece, it
+    does not."""
+    for k in range(3):
+        s, scale = gradient_case(rows, n, k, dtype, "cpu")
+        if s["weights"] is not None:
+            s["weights"][0] = 0.7
+        grad = oracle_policy(s, kl_coef=0.05)[2] * scale
+        rounded = f64(torch.from_numpy(grad).to(DTYPES[dtype]))
+        assert np.all(gradient_excess(s, rounded, scale) <= 0)
+        taken = np.zeros(grad.shape, bool)
+        taken[np.arange(rows), f64(s["actions"]).astype(int)] = True
+        only = gradient_excess(s, np.where(taken, rounded, 0.0), scale)
+        wanted = (grad != 0) & ~taken
+        assert np.mean(only[wanted] > 0) > 0.75, np.mean(only[wanted] > 0)
+        tail = rounded.copy()
+        tail[:, -8:] = np.where(taken, rounded, 0.0)[:, -8:]
+        assert np.any(gradient_excess(s, tail, scale) > 0)
+        assert np.any(gradient_excess(s, rounded * (1 + 1e-2), scale) > 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,n", POLICY_SIZES)
+def test_policy_loss_every_element_of_the_gradient(rows, n, dtype):
+    for k in range(3):
+        s, scale = gradient_case(rows, n, k, dtype, "cuda")
+        fused, auto, _ = fused_autograd_and_value(s, scale)
+        for r in (fused, auto):
+            check_gradient(s, r[2], scale)
+
+
+@pytest.mark.gpu
+def test_policy_loss_every_element_of_rows_read_twice():
+    """Rows longer than the registers hold, with a mask, in a padded buffer, and the rows that the test of offsets beyond 32 bits compares with."""
+    s = policy_inputs(3, 4, 70001, torch.bfloat16, "none", False, False, "cuda")
+    from diverse_conventions_amd import policy_loss_grad
+    check_gradient(s, policy_loss_grad(s["logits"], s["actions"], s["old"], s["adv"])[2], 1.0, kl_coef=0.0)
+    s = policy_inputs(5, 3, 70003, torch.float32, "rows", True, True, "cuda")
+    s["weights"][:] = 1.0
+    wide = torch.full((3, 70010), math.nan, device="cuda")
+    wide[:, 3:70006] = s["logits"]
+    s["logits"] = wide[:, 3:70006]
+    fused, auto, _ = fused_autograd_and_value(s)
+    for r in (fused, auto):
+        check_gradient(s, r[2], 1.0)
