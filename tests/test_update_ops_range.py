@@ -372,3 +372,39 @@ def test_policy_loss_every_element_of_rows_read_twice():
     fused, auto, _ = fused_autograd_and_value(s)
     for r in (fused, auto):
         check_gradient(s, r[2], 1.0)
+
+
+# ------------------------------------------------------------------------------------------------- the autograd forms in a graph
+@pytest.mark.gpu
+def test_losses_through_autograd_in_a_captured_graph():
+    """Forward and backward captured once and replayed on new inputs, eager calls and synchronisations between the replays."""
+    from diverse_conventions_amd import policy_loss, value_loss
+    small = policy_inputs(31, 9001, 6, device="cuda")
+    long = policy_inputs(32, 5, 5000, torch.bfloat16, device="cuda", available="none")
+    v, v0, ret, w = value_inputs(33, 9001, torch.float32, True, (1.0, 2.0))
+    leaves = [t.requires_grad_() for t in (small["logits"], long["logits"], v)]
+
+    def step():
+        out = []
+        for s in (small, long):
+            loss, stats = policy_loss(s["logits"], s["actions"], s["old"], s["adv"], kl_coef=0.05, ref_log_probs=s["ref"], active_masks=s["weights"],
+                                      available_actions=s["avail"])
+            out += [loss.detach(), stats, *torch.autograd.grad(loss * 3.0, s["logits"])]
+        loss = value_loss(v, v0, ret, active_masks=w, value_normalizer=(1.0, 2.0))
+        return out + [loss.detach(), *torch.autograd.grad(loss, v)]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        with torch.no_grad():
+            for t in leaves:
+                t.normal_()
+            small["weights"].uniform_()
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(seen, want)), k
