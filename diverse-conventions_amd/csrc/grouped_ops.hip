@@ -14,12 +14,13 @@
 // eight XCDs in contiguous runs: workgroups that share a network's weights share an L2.  (dW: every XCD gets its share of every group,
 // because a group's tiles cost what its rows are: 583 -> 387 us on ragged groups.)
 //
-// What bounds it (MI355X).  16-bit, 256 x 256 tiles: 4096^3 bf16 119 us = 1155 TFLOP/s (the library's product 1460); 16 ragged groups, 16 k
-// rows x 2048 x 4096: 323 us forward, 370 dx, 365 dw (the last round of tiles is half empty, a group's last tile too; even groups 300 us
-// forward = 917 TFLOP/s).  When the even forward took 304 us it took 258 without the matrix instructions, 220 without the copies and 295
-// without the LDS reads: the copies from L2 into LDS (8.5 TB/s over all CUs) and the wavefronts' meeting at two barriers a step bound it;
-// more steps in flight (3, 4), another order of the steps or cache hints on the copies change nothing.  f32: 4096^3 1034 us = 133 TFLOP/s
-// (library 915 us).  One to three rows a group: the weights' bytes, 252 MB in 58 us = 4.3 TB/s.
+// What bounds it (MI355X).  16-bit, 256 x 256 tiles: 4096^3 bf16 122 us = 1120 TFLOP/s (the library's product 1350); 16 ragged groups, 16 k
+// rows x 2048 x 4096: 323 - 329 us forward, 370 - 376 dx, 365 dw (the last round of tiles is half empty, a group's last tile too; even groups
+// 270 us forward = 1018 TFLOP/s).  The even forward takes 200 us without the copies, 234 without the matrix instructions, 261 without the LDS
+// reads and 260 without its stores: the copies from L2 into LDS (2.1 GB, 8 TB/s over all CUs) and the wavefronts' meeting at two barriers a
+// step bound it.  f32: 4096^3 1013 us = 136 TFLOP/s (library 150).  One to three rows a group: the weights' bytes, 252 MB in 58 us =
+// 4.3 TB/s.  Widths or addresses off 16 bytes go through registers one step ahead: 8192 rows of 2047 -> 2047 bf16 96 us forward and 517
+// backward, of 2048 -> 2048 64 and 152; f32 574 and 1211 against 515 and 1111.
 
 #include <hip/hip_runtime.h>
 
@@ -538,7 +539,7 @@ __global__ __launch_bounds__((BI / WI) * (BJ / WJ) * 64) void oc_grouped_kernel(
     if constexpr (sizeof(T) == 2) {
         if (a.splits == 1) {
             // 16-bit results go through LDS, rows of the tile in 16-byte pieces: as 8-byte pieces straight from the lanes, 32 bytes of a row
-            // at a time, the stores took 53 of 323 us (16 groups x 1024 rows x 2048 x 4096)
+            // at a time, 292 us instead of 270 (16 groups x 1024 rows x 2048 x 4096)
             constexpr int kPieces = BI / 8, kSpread = kPieces < 16 ? kPieces - 1 : 15;
             __syncthreads();                               // all have read the last step
 #pragma unroll

@@ -289,7 +289,7 @@ __device__ __forceinline__ float grad_of(const RowGrad &g, float v, float e) { r
 // -------------------------------------------------------------------------------------------------------------------------------
 // Up to 16 actions: a thread has a whole row.  The block's 256 rows are one contiguous piece of memory; it is copied through LDS in
 // 16-byte pieces, because lanes that each load their own 24 bytes touch every line of the piece once per load.  AM: so many values are
-// held in registers.  6.55 M rows of 6 f32 with gradient: 103 us (446 MB, 4.3 TB/s) and 14 us for the weights in front; 360 vector
+// held in registers.  6.55 M rows of 6 f32 with gradient: 106 us (446 MB, 4.2 TB/s) and 14 us for the weights in front; 360 vector
 // instructions a row with library logarithm, exponential and division made it 204 us.
 // -------------------------------------------------------------------------------------------------------------------------------
 constexpr int kRowTile = 256;
@@ -418,8 +418,8 @@ __global__ __launch_bounds__(256) void oc_policy_loss_rows_kernel(const PolicyLo
 // -------------------------------------------------------------------------------------------------------------------------------
 // More actions: L lanes have a row together, each C pieces of 16 bytes of it in registers (C = 0: more than fits, the row is read again
 // for the gradient).  One pass: a wavefront's maximum, its sums relative to that, and, where several wavefronts share the row, one
-// exchange of (maximum, sums) through LDS.  4096 rows of 32768 bf16 with gradient: 122 us, 4.4 TB/s, 85 % of a copy's rate: two
-// exponentials and 17 other vector instructions an element take 84 us, most of it under the memory's time.
+// exchange of (maximum, sums) through LDS.  4096 rows of 32768 bf16 with gradient: 128 us, 4.2 TB/s, 82 % of a copy's rate: two
+// exponentials and 19 other vector instructions an element, most of it under the memory's time (17, with one fma for an exponent: 124 us).
 // -------------------------------------------------------------------------------------------------------------------------------
 // Bits of -inf, in every element of a 32-bit word.  Pieces are put together as words: element by element the compiler gives each 16-bit
 // value a register of its own.
@@ -735,7 +735,7 @@ void launch_policy_loss(const PolicyLossArgs &a, hipStream_t s, int *blocks) {
         return dim3(*blocks);
     };
     // A row is held in registers up to 1024 lanes x 16 pieces: 64 K f32 or 128 K 16-bit actions.  Two rows or more a CU at once: 4096 pieces
-    // as 512 x 8 138 us, as 256 x 16 150 us (4096 x 32768 bf16, the weights added up in every block); 6253 pieces as 512 x 16 102 us, as 1024 x 8, one row a CU, 129 us
+    // as 512 x 8 or as 256 x 16 128 and 127 us (4096 x 32768 bf16); 6253 pieces as 512 x 16 103 us, as 1024 x 8, one row a CU, 122 us
     // (1023 x 50021 f16, forward and backward).
     const dim3 tiles = a.rows <= 2 * kRowTile ? dim3(1) : grid(kRowTile, kMaxBlocks);           // two tiles: one block, no launch to join
     if (a.rows <= 2 * kRowTile) *blocks = 1;
