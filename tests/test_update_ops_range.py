@@ -74,15 +74,13 @@ RANGES = [("all", f) for f in (1e9, -1e9, 1e10, -1e10, -1e20, 1e30, -1e30, -6e4)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("n", [6, 13, 40, 300, 5000, 40000, 140000])
-@pytest.mark.parametrize("kind,value", RANGES, ids=lambda v: v if isinstance(v, str) else f"{v:g}")
+@pytest.mark.parametrize("kind,value,dtype", [(k, v, d) for k, v in RANGES for d, t in DTYPES.items() if abs(v) <= torch.finfo(t).max],
+                         ids=lambda v: v if isinstance(v, str) else f"{v:g}")
 def test_policy_loss_of_logits_far_from_zero(kind, value, n, dtype):
     """Rows of one large value (uniform), a few ordinary logits among a finite fill (whole wavefronts and lanes see only the fill), all
     logits shifted: the loss is that of the differences, whatever they are relative to."""
     dt = DTYPES[dtype]
-    if abs(value) > torch.finfo(dt).max:
-        pytest.skip("not a value of the type")
     rows, scale = 3, 1024.0 if dtype == "f16" else 1.0
     s = policy_inputs(n + 1, rows, n, torch.float32, "none", False, True, "cuda")
     z = s["logits"]
